@@ -424,6 +424,221 @@ pplhip_retcode pplhip_check_tables(const pplhip_mhca_args* args, int64_t max_sla
  * is 2 x int32 in host memory, and no device is touched. */
 pplhip_retcode pplhip_check_tables_host(const pplhip_mhca_args* args, int64_t max_slab_tokens, int32_t* flag);
 
+/*
+ * Attention of drafted token trees over the int8 slab (speculative decoding: a step verifies a tree of drafted tokens per
+ * sequence in one call). The reference has no such operator; its MultiHeadCacheAttention could express one only through
+ * a dense [tokens, keys of the whole batch] attn_mask. Also serves plain decode steps and chunks of a prompt over the
+ * slab (d_tree_mask NULL), with the log-sums that pplhip_kv_score_accumulate takes.
+ *
+ *   query      fp16 [S, num_heads, head_dim]       S = seqstarts[batch] packed new (drafted) tokens
+ *   tree_mask  u64  [S, tree_mask_words]           bit i % 64 of word i / 64 of row t: token t sees the i-th new token of
+ *                                                  its own sequence (itself included if its bit is set); bits at or past
+ *                                                  the sequence's token count are ignored. NULL: token t sees the new
+ *                                                  tokens 0 .. t of its sequence (tree_mask_words is not read)
+ *   output     fp16 [S, num_heads, head_dim]
+ *   lse        f32  [S, num_heads] or NULL         natural logarithm of the sum of exp(score) over the visible keys
+ * Sequence b has L = seqstarts[b+1] - seqstarts[b] new tokens (0 allowed) and kvstarts[b+1] - kvstarts[b] cached ones,
+ * of which the last L are the new tokens themselves: the slab must already hold them (pplhip_kv_quantize_write or
+ * pplhip_rope_kv_write_forward put them there). A token sees every cached token in front of the new ones, and of the
+ * new ones those its mask row names; score = q . k / sqrt(head_dim). A row that sees nothing yields zeros and -inf.
+ * Keys a row does not see contribute nothing to it, whatever the slab holds for them (NaN and infinities included).
+ * Rows of query / output at or past seqstarts[batch] are neither read nor written.
+ * head_dim: a multiple of 16 up to 256; any num_heads that num_kv_heads divides; cache layouts, pages and strides as
+ * for pplhip_mhca_args. Drafted tokens' rotary positions (start + depth in the tree) are not those of a run of
+ * consecutive tokens: pplhip_rope_forward takes one-token sequences (batch = S, seqstarts 0 .. S) with
+ * start_pos = the tokens' positions.
+ */
+typedef struct pplhip_tree_attention_args {
+    const void* d_query;
+    const uint64_t* d_tree_mask;
+    const int64_t* d_seqstarts; /* [batch+1] */
+    const int64_t* d_kvstarts; /* [batch+1] */
+    const int64_t* d_cachestarts; /* [batch], or the [batch, cachestart_stride_b] page table */
+    int64_t batch;
+    int64_t total_new_tokens; /* rows of query; at least seqstarts[batch] */
+    int64_t max_seqlen; /* longest sequence's new tokens */
+    int64_t max_kvlen; /* longest sequence's cached tokens, the new ones included */
+    int32_t tree_mask_words; /* at least ceil(max_seqlen / 64) */
+    int32_t layer_idx;
+    int32_t num_layer;
+    int32_t num_heads;
+    int32_t num_kv_heads;
+    int32_t head_dim;
+    int32_t cache_mode;
+    int32_t page_size;
+    int64_t cache_stride_s;
+    int64_t cache_stride_l;
+    int64_t cache_stride_h;
+    int64_t cache_stride_kv;
+    int64_t cachestart_stride_b;
+    const void* d_cache;
+    const void* d_scale;
+    void* d_output;
+    void* d_lse;
+} pplhip_tree_attention_args;
+
+/* Filled by pplhip_tree_attention_prepare for one argument block; prepare again when batch, total_new_tokens, max_seqlen,
+ * max_kvlen, the head counts or head_dim change. */
+typedef struct pplhip_tree_attention_plan {
+    uint64_t workspace_bytes; /* device scratch the caller passes to forward, 256-byte aligned (may be 0) */
+    int32_t num_ranges; /* equal shares the keys of all (sequence, row tile) pairs are cut into on the device */
+    int32_t row_tile; /* (token, query head of the kv head) rows a workgroup takes */
+} pplhip_tree_attention_plan;
+
+/* Host-only, like pplhip_mhca_prepare. */
+pplhip_retcode pplhip_tree_attention_prepare(const pplhip_tree_attention_args* args, pplhip_tree_attention_plan* plan);
+/* Enqueues at most two launches (attention, merge of split results), allocates nothing; capturable. Calls that overlap
+ * in time (two streams, two captured graphs) need a workspace each. */
+pplhip_retcode pplhip_tree_attention_forward(const pplhip_tree_attention_args* args,
+                                             const pplhip_tree_attention_plan* plan, void* d_workspace, void* stream);
+
+/*
+ * Accumulated attention weight of every cached token, kept per kv head (the measure pplhip_kv_evict goes by):
+ *   score_out[head][tok(j)] = (j < start ? score_in[head][tok(j)] : 0)
+ *                             + sum over the sequence's new tokens t >= j - start and the query heads h of the kv head of
+ *                               exp(q_th . k_j / sqrt(head_dim) - lse[t][h])
+ * for every cached token j of every sequence (start = cached tokens in front of the new ones; a new token's sum starts
+ * from 0), with the log-sums of pplhip_tree_attention_forward. New tokens see each other causally; after a tree step
+ * the caller passes the accepted tokens' rows (which pplhip_kv_accept has made a run of tokens). A row whose lse is
+ * -inf saw nothing and adds nothing. score_in and score_out may be the same array.
+ * position_idx (i64 [S], what pplhip_position_index yields) is stored as i32 in `position` for the new tokens; both NULL
+ * when no positions are kept.
+ *   score_in / score_out f32, position i32: element [layer][head][slab token] at
+ *     layer * score_stride_l + head * score_stride_h + slab token
+ * Sequences without new tokens are left out: their score_out entries are not written.
+ * The sums' order is fixed: equal inputs give equal bits.
+ */
+typedef struct pplhip_kv_score_args {
+    const void* d_query; /* fp16 [S, num_heads, head_dim] */
+    const void* d_lse; /* f32 [S, num_heads] */
+    const int64_t* d_position_idx; /* i64 [S] or NULL */
+    const int64_t* d_seqstarts; /* [batch+1] */
+    const int64_t* d_kvstarts; /* [batch+1] */
+    const int64_t* d_cachestarts;
+    int64_t batch;
+    int64_t total_new_tokens;
+    int64_t max_seqlen;
+    int64_t max_kvlen;
+    int32_t layer_idx;
+    int32_t num_layer;
+    int32_t num_heads;
+    int32_t num_kv_heads;
+    int32_t head_dim;
+    int32_t cache_mode;
+    int32_t page_size;
+    int32_t reserved;
+    int64_t cache_stride_s;
+    int64_t cache_stride_l;
+    int64_t cache_stride_h;
+    int64_t cache_stride_kv;
+    int64_t cachestart_stride_b;
+    const void* d_cache;
+    const void* d_scale;
+    const float* d_score_in;
+    float* d_score_out;
+    int32_t* d_position; /* or NULL */
+    int64_t score_stride_l;
+    int64_t score_stride_h;
+} pplhip_kv_score_args;
+
+pplhip_retcode pplhip_kv_score_accumulate(const pplhip_kv_score_args* args, void* stream);
+
+/*
+ * Eviction from the cache by accumulated attention weight. For every sequence b, layer layer_idx .. layer_idx +
+ * layer_count - 1 and kv head on its own, K = min(kvlen, max(target_kvlen[b], 0)) of the kvlen cached tokens stay:
+ * first those whose position is below num_sink or at least next_pos[b] - num_recent, then those with the largest score;
+ * a NaN score counts as the smallest, ties go to the lower index. Tokens with index below K that stay are left where
+ * they are; the j-th token (ascending) with index below K that goes has its slab row (int8 K and V, scales, score,
+ * position) overwritten by that of the j-th from last staying token with index K or more. Slab rows, scores and
+ * positions at index K and beyond are left as they were. So the kept tokens end up in the first K places, in an order
+ * that attention does not depend on (keys are cached rotated); `position` says which token of the text a place holds.
+ * new_kvlen[b] = K.
+ * score_in / score_out and position_in / position_out are laid out as for pplhip_kv_score_accumulate; each pair may be
+ * the same array (in place), otherwise the out arrays get entries 0 .. K-1 of every sequence and the in arrays are left
+ * alone. position_in and position_out may both be NULL when num_sink and num_recent are 0.
+ * Scores or positions of different sequences must not overlap, nor their slab regions.
+ */
+typedef struct pplhip_kv_evict_args {
+    const int64_t* d_kvstarts; /* [batch+1] */
+    const int64_t* d_cachestarts;
+    const int64_t* d_target_kvlen; /* [batch] */
+    const int64_t* d_next_pos; /* [batch]: position the sequence's next token will have; NULL if num_recent is 0 */
+    int64_t batch;
+    int64_t max_kvlen;
+    int32_t num_sink;
+    int32_t num_recent;
+    int32_t layer_idx; /* first layer */
+    int32_t layer_count;
+    int32_t num_layer;
+    int32_t num_kv_heads;
+    int32_t head_dim;
+    int32_t cache_mode;
+    int32_t page_size;
+    int32_t reserved;
+    int64_t cache_stride_s;
+    int64_t cache_stride_l;
+    int64_t cache_stride_h;
+    int64_t cache_stride_kv;
+    int64_t cachestart_stride_b;
+    void* d_cache;
+    void* d_scale;
+    const float* d_score_in;
+    float* d_score_out;
+    const int32_t* d_position_in;
+    int32_t* d_position_out;
+    int64_t score_stride_l;
+    int64_t score_stride_h;
+    int64_t* d_new_kvlen; /* [batch] */
+} pplhip_kv_evict_args;
+
+typedef struct pplhip_kv_evict_plan {
+    uint64_t workspace_bytes; /* device scratch the caller passes to evict, 256-byte aligned (may be 0) */
+    int32_t max_moves; /* rows one (sequence, layer, kv head) can have to move: max_kvlen / 2 */
+    int32_t reserved;
+} pplhip_kv_evict_plan;
+
+/* Host-only. */
+pplhip_retcode pplhip_kv_evict_prepare(const pplhip_kv_evict_args* args, pplhip_kv_evict_plan* plan);
+/* Enqueues two launches (choice, move), allocates nothing; capturable. Overlapping calls need a workspace each. */
+pplhip_retcode pplhip_kv_evict(const pplhip_kv_evict_args* args, const pplhip_kv_evict_plan* plan, void* d_workspace,
+                               void* stream);
+
+/*
+ * Keeps the accepted path of a verified draft: slab row start_pos[b] + i of every layer layer_idx .. layer_idx +
+ * layer_count - 1, K and V, all kv heads, becomes what row start_pos[b] + accepted[b * accepted_stride_b + i] was
+ * before the call, i = 0 .. accepted_len[b] - 1. A sequence's list names its drafted tokens in ascending order (a
+ * tree's parents precede their children); the list is taken to end at the first entry that is not larger than the one
+ * before it or lies outside [0, seqlen_b), and at max_accepted entries. Rows behind the path keep their contents.
+ */
+typedef struct pplhip_kv_accept_args {
+    const int64_t* d_seqstarts; /* [batch+1]: seqlen_b drafted tokens */
+    const int64_t* d_start_pos; /* [batch]: cached tokens in front of them */
+    const int64_t* d_cachestarts;
+    const int64_t* d_accepted; /* [batch, accepted_stride_b] */
+    const int64_t* d_accepted_len; /* [batch] */
+    int64_t accepted_stride_b;
+    int64_t max_accepted;
+    int64_t batch;
+    int32_t layer_idx; /* first layer */
+    int32_t layer_count;
+    int32_t num_layer;
+    int32_t num_kv_heads;
+    int32_t head_dim;
+    int32_t cache_mode;
+    int32_t page_size;
+    int32_t reserved;
+    int64_t cache_stride_s;
+    int64_t cache_stride_l;
+    int64_t cache_stride_h;
+    int64_t cache_stride_kv;
+    int64_t cachestart_stride_b;
+    void* d_cache;
+    void* d_scale;
+} pplhip_kv_accept_args;
+
+/* One launch; allocates nothing, needs no workspace. */
+pplhip_retcode pplhip_kv_accept(const pplhip_kv_accept_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

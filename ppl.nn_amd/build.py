@@ -10,7 +10,8 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 # attention.hip is decode.hip + prefill.hip in one translation unit (it includes them: a call with decode sequences and
 # prompts runs both kinds of workgroup in one launch)
-KERNEL_SOURCES = ["api.hip", "kv_quant.hip", "attention.hip", "pack.hip", "rope.hip", "generic.hip"]
+KERNEL_SOURCES = ["api.hip", "kv_quant.hip", "attention.hip", "pack.hip", "rope.hip", "generic.hip",
+                  "tree.hip", "score.hip", "evict.hip"]
 KERNEL_INCLUDED = ["decode.hip", "prefill.hip"]
 
 HIP_FLAGS = [
@@ -37,7 +38,7 @@ def build_kernels(force=False, verbose=False, conservative_waits=False):
     tag = "_conservative_waits" if conservative_waits else ""
     out = os.path.join(LIBDIR, f"libppl_llm_kernel_hip{tag}.so")
     srcs = [os.path.join(CSRC, s) for s in KERNEL_SOURCES]
-    deps = srcs + [os.path.join(CSRC, s) for s in KERNEL_INCLUDED] + [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "table_check.h"), os.path.join(CSRC, "exports.map"),
+    deps = srcs + [os.path.join(CSRC, s) for s in KERNEL_INCLUDED] + [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "cache_tile.h"), os.path.join(CSRC, "table_check.h"), os.path.join(CSRC, "exports.map"),
                    os.path.join(HERE, "..", "include", "ppl_llm_kernel_hip.h")]
     if not force and not _newer(out, deps):
         return out

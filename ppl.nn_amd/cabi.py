@@ -115,6 +115,69 @@ class PackArgs(C.Structure):
     ]
 
 
+_CACHE_TAIL = [
+    ("cache_mode", _i32), ("page_size", _i32),
+]
+_CACHE_STRIDES = [
+    ("cache_stride_s", _i64), ("cache_stride_l", _i64), ("cache_stride_h", _i64), ("cache_stride_kv", _i64),
+    ("cachestart_stride_b", _i64),
+    ("d_cache", _p), ("d_scale", _p),
+]
+
+
+class TreeAttentionArgs(C.Structure):
+    _fields_ = [
+        ("d_query", _p), ("d_tree_mask", _p),
+        ("d_seqstarts", _p), ("d_kvstarts", _p), ("d_cachestarts", _p),
+        ("batch", _i64), ("total_new_tokens", _i64), ("max_seqlen", _i64), ("max_kvlen", _i64),
+        ("tree_mask_words", _i32), ("layer_idx", _i32), ("num_layer", _i32), ("num_heads", _i32),
+        ("num_kv_heads", _i32), ("head_dim", _i32),
+    ] + _CACHE_TAIL + _CACHE_STRIDES + [
+        ("d_output", _p), ("d_lse", _p),
+    ]
+
+
+class TreeAttentionPlan(C.Structure):
+    _fields_ = [("workspace_bytes", C.c_uint64), ("num_ranges", _i32), ("row_tile", _i32)]
+
+
+class KvScoreArgs(C.Structure):
+    _fields_ = [
+        ("d_query", _p), ("d_lse", _p), ("d_position_idx", _p),
+        ("d_seqstarts", _p), ("d_kvstarts", _p), ("d_cachestarts", _p),
+        ("batch", _i64), ("total_new_tokens", _i64), ("max_seqlen", _i64), ("max_kvlen", _i64),
+        ("layer_idx", _i32), ("num_layer", _i32), ("num_heads", _i32), ("num_kv_heads", _i32), ("head_dim", _i32),
+    ] + _CACHE_TAIL + [("reserved", _i32)] + _CACHE_STRIDES + [
+        ("d_score_in", _p), ("d_score_out", _p), ("d_position", _p),
+        ("score_stride_l", _i64), ("score_stride_h", _i64),
+    ]
+
+
+class KvEvictArgs(C.Structure):
+    _fields_ = [
+        ("d_kvstarts", _p), ("d_cachestarts", _p), ("d_target_kvlen", _p), ("d_next_pos", _p),
+        ("batch", _i64), ("max_kvlen", _i64),
+        ("num_sink", _i32), ("num_recent", _i32),
+        ("layer_idx", _i32), ("layer_count", _i32), ("num_layer", _i32), ("num_kv_heads", _i32), ("head_dim", _i32),
+    ] + _CACHE_TAIL + [("reserved", _i32)] + _CACHE_STRIDES + [
+        ("d_score_in", _p), ("d_score_out", _p), ("d_position_in", _p), ("d_position_out", _p),
+        ("score_stride_l", _i64), ("score_stride_h", _i64),
+        ("d_new_kvlen", _p),
+    ]
+
+
+class KvEvictPlan(C.Structure):
+    _fields_ = [("workspace_bytes", C.c_uint64), ("max_moves", _i32), ("reserved", _i32)]
+
+
+class KvAcceptArgs(C.Structure):
+    _fields_ = [
+        ("d_seqstarts", _p), ("d_start_pos", _p), ("d_cachestarts", _p), ("d_accepted", _p), ("d_accepted_len", _p),
+        ("accepted_stride_b", _i64), ("max_accepted", _i64), ("batch", _i64),
+        ("layer_idx", _i32), ("layer_count", _i32), ("num_layer", _i32), ("num_kv_heads", _i32), ("head_dim", _i32),
+    ] + _CACHE_TAIL + [("reserved", _i32)] + _CACHE_STRIDES
+
+
 # name -> (restype, argtypes); every symbol the header declares
 PROTOTYPES = {
     "pplhip_last_error": (C.c_char_p, []),
@@ -133,6 +196,12 @@ PROTOTYPES = {
     "pplhip_advance_slots": (_i32, [_p, _p, _i32, _p]),
     "pplhip_check_tables": (_i32, [C.POINTER(MhcaArgs), _i64, _p, _p]),
     "pplhip_check_tables_host": (_i32, [C.POINTER(MhcaArgs), _i64, _p]),
+    "pplhip_tree_attention_prepare": (_i32, [C.POINTER(TreeAttentionArgs), C.POINTER(TreeAttentionPlan)]),
+    "pplhip_tree_attention_forward": (_i32, [C.POINTER(TreeAttentionArgs), C.POINTER(TreeAttentionPlan), _p, _p]),
+    "pplhip_kv_score_accumulate": (_i32, [C.POINTER(KvScoreArgs), _p]),
+    "pplhip_kv_evict_prepare": (_i32, [C.POINTER(KvEvictArgs), C.POINTER(KvEvictPlan)]),
+    "pplhip_kv_evict": (_i32, [C.POINTER(KvEvictArgs), C.POINTER(KvEvictPlan), _p, _p]),
+    "pplhip_kv_accept": (_i32, [C.POINTER(KvAcceptArgs), _p]),
 }
 
 # the measurement / verification aids of libppl_llm_kernel_hip_probes.so (include/ppl_llm_kernel_hip_probes.h)

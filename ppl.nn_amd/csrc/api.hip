@@ -150,6 +150,41 @@ static pplhip_retcode validate_write(const pplhip_kv_write_args* a) {
     return PPLHIP_RC_SUCCESS;
 }
 
+// what the four operators check of the slab they work on (layer_count: 1 for those of one layer)
+template <class Args>
+static pplhip_retcode validate_slab(const Args* a, int layer_count) {
+    const pplhip_retcode rc = validate_common(a->num_kv_heads, a->head_dim, a->num_layer, a->layer_idx, a->cache_stride_s,
+                                              a->cache_stride_l, a->cache_stride_h, a->cache_stride_kv, a->d_cache,
+                                              a->d_scale);
+    if (rc != PPLHIP_RC_SUCCESS) return rc;
+    if (layer_count < 1 || layer_count > a->num_layer - a->layer_idx)
+        PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "layers %d .. %lld of %d", a->layer_idx,
+                    (long long)a->layer_idx + layer_count - 1, a->num_layer);
+    if (a->batch < 0) PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "negative batch");
+    if (a->batch > 0x7fffffffLL) PPLHIP_FAIL(PPLHIP_RC_OUT_OF_RANGE, "too many sequences");
+    return validate_cache_mode(a->cache_mode, a->page_size, a->cachestart_stride_b);
+}
+
+// the packed queries and their tables; *empty: no sequences or no tokens
+template <class Args>
+static pplhip_retcode validate_queries(const Args* a, bool* empty) {
+    *empty = false;
+    if (a->num_heads <= 0 || a->num_kv_heads <= 0 || a->num_heads % a->num_kv_heads)
+        PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "num_heads %d is not a multiple of num_kv_heads %d", a->num_heads,
+                    a->num_kv_heads);
+    if (a->total_new_tokens < 0 || a->max_seqlen < 0 || a->max_seqlen > a->total_new_tokens || a->max_kvlen < a->max_seqlen)
+        PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "inconsistent sizes: tokens %lld max_seqlen %lld max_kvlen %lld",
+                    (long long)a->total_new_tokens, (long long)a->max_seqlen, (long long)a->max_kvlen);
+    if (a->batch == 0 || a->total_new_tokens == 0 || a->max_seqlen == 0) {
+        *empty = true;
+        return PPLHIP_RC_SUCCESS;
+    }
+    if (!a->d_query || !a->d_seqstarts || !a->d_kvstarts || !a->d_cachestarts)
+        PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "null tensor pointer");
+    if ((uintptr_t)a->d_query & 15) PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "query must be 16-byte aligned");
+    return PPLHIP_RC_SUCCESS;
+}
+
 } // namespace pplhip
 
 using namespace pplhip;
@@ -161,7 +196,7 @@ const char* pplhip_last_error(void) {
 }
 
 int32_t pplhip_version(void) {
-    return 300; // 0.3.0
+    return 400; // 0.4.0
 }
 
 pplhip_retcode pplhip_init(void) {
@@ -517,6 +552,128 @@ pplhip_retcode pplhip_advance_slots(int64_t* d_slot_kvlen, const int64_t* d_slot
     if (num_slots < 0 || (num_slots > 0 && (!d_slot_kvlen || !d_slot_newlen)))
         PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "bad slot arrays");
     return launch_advance_slots(d_slot_kvlen, d_slot_newlen, num_slots, (hipStream_t)stream);
+}
+
+// ---- several new tokens over the slab, and the cache's upkeep
+
+static pplhip_retcode validate_tree(const pplhip_tree_attention_args* a, bool* empty) {
+    pplhip_retcode rc = validate_slab(a, 1);
+    if (rc != PPLHIP_RC_SUCCESS) return rc;
+    rc = validate_queries(a, empty);
+    if (rc != PPLHIP_RC_SUCCESS || *empty) return rc;
+    if (!a->d_output) PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "null tensor pointer");
+    if (((uintptr_t)a->d_output & 15) || ((uintptr_t)a->d_lse & 3) || ((uintptr_t)a->d_tree_mask & 7))
+        PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "output must be 16-byte, lse 4-byte, tree_mask 8-byte aligned");
+    if (a->d_tree_mask && (a->tree_mask_words <= 0 || (a->max_seqlen + 63) / 64 > a->tree_mask_words))
+        PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "tree_mask_words %d: %lld tokens need %lld", a->tree_mask_words,
+                    (long long)a->max_seqlen, (long long)((a->max_seqlen + 63) / 64));
+    return PPLHIP_RC_SUCCESS;
+}
+
+pplhip_retcode pplhip_tree_attention_prepare(const pplhip_tree_attention_args* a, pplhip_tree_attention_plan* plan) {
+    if (!a || !plan) PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "null argument block");
+    memset(plan, 0, sizeof(*plan));
+    bool empty;
+    const pplhip_retcode rc = validate_tree(a, &empty);
+    if (rc != PPLHIP_RC_SUCCESS || empty) return rc;
+    plan->row_tile = tree_row_tile(a);
+    plan->num_ranges = (int32_t)tree_num_ranges(a, device_cu_count());
+    plan->workspace_bytes = (tree_workspace_bytes(a, plan->num_ranges) + 255) / 256 * 256;
+    return PPLHIP_RC_SUCCESS;
+}
+
+pplhip_retcode pplhip_tree_attention_forward(const pplhip_tree_attention_args* a, const pplhip_tree_attention_plan* plan,
+                                             void* d_workspace, void* stream) {
+    if (!a || !plan) PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "null argument block");
+    bool empty;
+    const pplhip_retcode rc = validate_tree(a, &empty);
+    if (rc != PPLHIP_RC_SUCCESS || empty) return rc;
+    if (plan->num_ranges <= 0 || (int64_t)plan->num_ranges * a->num_kv_heads > 0x7fffffffLL ||
+        plan->row_tile != tree_row_tile(a) || tree_workspace_bytes(a, plan->num_ranges) > plan->workspace_bytes)
+        PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "plan was not produced by pplhip_tree_attention_prepare for these arguments");
+    if (!d_workspace || ((uintptr_t)d_workspace & 255))
+        PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "workspace of %llu bytes (256-byte aligned) required",
+                    (unsigned long long)plan->workspace_bytes);
+    return launch_tree_attention(a, plan->num_ranges, d_workspace, (hipStream_t)stream);
+}
+
+pplhip_retcode pplhip_kv_score_accumulate(const pplhip_kv_score_args* a, void* stream) {
+    if (!a) PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "null argument block");
+    pplhip_retcode rc = validate_slab(a, 1);
+    if (rc != PPLHIP_RC_SUCCESS) return rc;
+    bool empty;
+    rc = validate_queries(a, &empty);
+    if (rc != PPLHIP_RC_SUCCESS) return rc;
+    if (a->score_stride_l < 0 || a->score_stride_h < 0)
+        PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "negative score strides");
+    if ((a->d_position != nullptr) != (a->d_position_idx != nullptr))
+        PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "position and position_idx: both or neither");
+    if (empty) return PPLHIP_RC_SUCCESS;
+    if (!a->d_lse || !a->d_score_in || !a->d_score_out) PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "null tensor pointer");
+    if (((uintptr_t)a->d_lse & 3) || ((uintptr_t)a->d_score_in & 3) || ((uintptr_t)a->d_score_out & 3) ||
+        ((uintptr_t)a->d_position & 3) || ((uintptr_t)a->d_position_idx & 7))
+        PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "lse, score and position must be 4-byte, position_idx 8-byte aligned");
+    return launch_kv_score(a, (hipStream_t)stream);
+}
+
+static pplhip_retcode validate_evict(const pplhip_kv_evict_args* a) {
+    const pplhip_retcode rc = validate_slab(a, a->layer_count);
+    if (rc != PPLHIP_RC_SUCCESS) return rc;
+    if (a->num_sink < 0 || a->num_recent < 0) PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "negative num_sink or num_recent");
+    if (a->max_kvlen < 0) PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "negative max_kvlen");
+    if (a->score_stride_l < 0 || a->score_stride_h < 0)
+        PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "negative score strides");
+    if ((a->d_position_in != nullptr) != (a->d_position_out != nullptr))
+        PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "position_in and position_out: both or neither");
+    if ((a->num_sink > 0 || a->num_recent > 0) && !a->d_position_in)
+        PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "num_sink and num_recent need the tokens' positions");
+    if (a->max_kvlen > 0x7fffffffLL || (double)a->batch * a->layer_count * a->num_kv_heads > 2147483647.0)
+        PPLHIP_FAIL(PPLHIP_RC_OUT_OF_RANGE, "kv_evict: too many tokens or (sequence, layer, kv head) columns");
+    if (a->batch == 0) return PPLHIP_RC_SUCCESS;
+    if (!a->d_kvstarts || !a->d_cachestarts || !a->d_target_kvlen || !a->d_score_in || !a->d_score_out || !a->d_new_kvlen ||
+        (a->num_recent > 0 && !a->d_next_pos))
+        PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "null tensor pointer");
+    if (((uintptr_t)a->d_score_in & 3) || ((uintptr_t)a->d_score_out & 3) || ((uintptr_t)a->d_position_in & 3) ||
+        ((uintptr_t)a->d_position_out & 3))
+        PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "score and position must be 4-byte aligned");
+    return PPLHIP_RC_SUCCESS;
+}
+
+pplhip_retcode pplhip_kv_evict_prepare(const pplhip_kv_evict_args* a, pplhip_kv_evict_plan* plan) {
+    if (!a || !plan) PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "null argument block");
+    memset(plan, 0, sizeof(*plan));
+    const pplhip_retcode rc = validate_evict(a);
+    if (rc != PPLHIP_RC_SUCCESS) return rc;
+    plan->max_moves = (int32_t)(a->max_kvlen / 2); // rows that move are at most those that stay and those that go
+    plan->workspace_bytes = (evict_workspace_bytes(a, plan->max_moves) + 255) / 256 * 256;
+    return PPLHIP_RC_SUCCESS;
+}
+
+pplhip_retcode pplhip_kv_evict(const pplhip_kv_evict_args* a, const pplhip_kv_evict_plan* plan, void* d_workspace,
+                               void* stream) {
+    if (!a || !plan) PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "null argument block");
+    const pplhip_retcode rc = validate_evict(a);
+    if (rc != PPLHIP_RC_SUCCESS) return rc;
+    if (a->batch == 0) return PPLHIP_RC_SUCCESS;
+    if (plan->max_moves < a->max_kvlen / 2 || evict_workspace_bytes(a, plan->max_moves) > plan->workspace_bytes)
+        PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "plan was not produced by pplhip_kv_evict_prepare for these arguments");
+    if (!d_workspace || ((uintptr_t)d_workspace & 255))
+        PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "workspace of %llu bytes (256-byte aligned) required",
+                    (unsigned long long)plan->workspace_bytes);
+    return launch_kv_evict(a, plan->max_moves, d_workspace, (hipStream_t)stream);
+}
+
+pplhip_retcode pplhip_kv_accept(const pplhip_kv_accept_args* a, void* stream) {
+    if (!a) PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "null argument block");
+    const pplhip_retcode rc = validate_slab(a, a->layer_count);
+    if (rc != PPLHIP_RC_SUCCESS) return rc;
+    if (a->max_accepted < 0 || a->accepted_stride_b < a->max_accepted)
+        PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "max_accepted %lld, accepted_stride_b %lld", (long long)a->max_accepted,
+                    (long long)a->accepted_stride_b);
+    if (a->batch == 0 || a->max_accepted == 0) return PPLHIP_RC_SUCCESS;
+    if (!a->d_seqstarts || !a->d_start_pos || !a->d_cachestarts || !a->d_accepted || !a->d_accepted_len)
+        PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "null table pointer");
+    return launch_kv_accept(a, (hipStream_t)stream);
 }
 
 } // extern "C"

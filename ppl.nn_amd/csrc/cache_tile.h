@@ -1,0 +1,114 @@
+// How a wave brings 32 consecutive cached rows (one kv head's K or V) from the int8 slab into LDS as fp16, for the kernels
+// that feed them to the matrix cores (tree.hip, score.hip).
+//
+// A lane loads 16-byte pieces (two quantisation groups), consecutive lanes consecutive pieces of a row, so that one load
+// instruction covers whole 128-byte lines, and with them the two groups' scales (4 bytes). Dequantisation happens in that
+// orientation, where a group's scale is one value: fp16(float(q) * float(scale)), as everywhere. Rows have DH channels in
+// LDS (head_dim rounded up to a multiple of 32, zeros past head_dim) and are padded by 8 halves: 16-byte reads of 16
+// rows at one column, and the writes, then touch every bank once.
+#ifndef PPLHIP_CSRC_CACHE_TILE_H_
+#define PPLHIP_CSRC_CACHE_TILE_H_
+
+#include "common.h"
+
+namespace pplhip {
+
+typedef uint32_t uint4_vt __attribute__((ext_vector_type(4)));
+typedef const int64_t __attribute__((address_space(4)))* const_tab64_t; // wave-uniform reads are scalar loads
+
+constexpr int kTileKeys = 32;
+
+// Where a call's cached rows are; the same for every workgroup.
+struct CacheView {
+    const int8_t* cache;
+    const half_t* scale;
+    const int64_t* cachestarts;
+    int64_t cs_stride_b;
+    CacheAddr addr;
+    int32_t page_shift; // 0: contiguous region per sequence
+    int32_t head_dim;
+
+    // element offset of the K row of key j of sequence b (both wave-uniform; a run of 32 keys from a multiple of 32
+    // lies in one page: pages are powers of two of at least 64 tokens)
+    __device__ inline int64_t key_row(int64_t b, int64_t j, int kvh) const {
+        const const_tab64_t tab = (const_tab64_t)cachestarts;
+        const int64_t t = page_shift == 0 ? tab[b] + j
+                                          : tab[b * cs_stride_b + (j >> page_shift)] +
+                                                (j & ((int64_t(1) << page_shift) - 1));
+        return addr.row(t, 0, kvh);
+    }
+};
+
+inline int padded_head_dim(int head_dim) { // the kernels' DH
+    return (head_dim + 31) / 32 * 32;
+}
+
+// The wave's LDS operations keep their order by themselves; this only tells the compiler that lanes read what other
+// lanes of the wave wrote.
+__device__ inline void wave_lds_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+template <int DH>
+struct CacheTile {
+    static constexpr int PIECES = DH / 16; // 16-byte pieces of a row
+    static constexpr int NLD = DH / 32; // pieces a lane loads
+    static constexpr int LDR = DH + 8; // halves per LDS row
+    uint4_vt q[NLD];
+    uint32_t s[NLD];
+
+    // rows kv0 .. kv0 + 31 from element offset `base`; rows past the sequence's last key (kvlen - 1) repeat it, so that
+    // nothing unwritten is ever multiplied
+    __device__ inline void fetch(const CacheView& v, int64_t base, int64_t kv0, int64_t kvlen) {
+        const int lane = threadIdx.x & 63;
+        const int64_t n_left = kvlen - kv0;
+        const int last = n_left < kTileKeys ? (int)n_left - 1 : kTileKeys - 1;
+        const char* cbase = (const char*)v.cache + base;
+        const char* sbase = (const char*)v.scale + base / 4; // one fp16 per 8 channels
+#pragma unroll
+        for (int n = 0; n < NLD; ++n) {
+            const int c = lane + 64 * n;
+            const int row = c / PIECES, piece = c - row * PIECES;
+            // (token strides are below 2^25 elements: 32 of them fit 32 bits)
+            const uint32_t off = (uint32_t)(row < last ? row : last) * (uint32_t)v.addr.stride_s + 16u * piece;
+            if (16 * piece < v.head_dim) {
+                q[n] = __builtin_nontemporal_load(reinterpret_cast<const uint4_vt*>(cbase + off));
+                s[n] = *reinterpret_cast<const uint32_t*>(sbase + off / 4);
+            } else { // channels past head_dim
+                q[n] = uint4_vt{0, 0, 0, 0};
+                s[n] = 0;
+            }
+        }
+    }
+
+    __device__ inline void stash(half_t* tile) const {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int n = 0; n < NLD; ++n) {
+            const int c = lane + 64 * n;
+            const int row = c / PIECES, piece = c - row * PIECES;
+            const half2_t s2 = as_half2(s[n]);
+            half8_t* dst = reinterpret_cast<half8_t*>(tile + row * LDR + 16 * piece);
+            dst[0] = dequant8(q[n].x, q[n].y, s2.x);
+            dst[1] = dequant8(q[n].z, q[n].w, s2.y);
+        }
+    }
+
+    // bit r: row r may hold a value that is not finite (|int8| <= 128, and 128 * 511 is below fp16's largest)
+    __device__ inline uint32_t odd_rows() const {
+        uint32_t rows = 0;
+#pragma unroll
+        for (int n = 0; n < NLD; ++n) {
+            const half2_t s2 = as_half2(s[n]);
+            const bool fine = __builtin_fabsf((float)s2.x) < 511.f && __builtin_fabsf((float)s2.y) < 511.f;
+            for (uint64_t bad = __ballot(!fine); bad; bad &= bad - 1)
+                rows |= 1u << ((__builtin_ctzll(bad) + 64 * n) / PIECES);
+        }
+        return rows;
+    }
+};
+
+} // namespace pplhip
+
+#endif

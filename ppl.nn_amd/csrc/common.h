@@ -204,6 +204,16 @@ pplhip_retcode launch_pack_tables(const pplhip_pack_args* a, hipStream_t stream)
 pplhip_retcode launch_advance_slots(int64_t* kvlen, const int64_t* newlen, int n, hipStream_t stream);
 pplhip_retcode launch_check_tables(const pplhip_mhca_args* a, int64_t max_slab_tokens, int32_t* d_flag, hipStream_t stream);
 void check_tables_host(const pplhip_mhca_args* a, int64_t max_slab_tokens, int32_t* flag);
+// several new tokens per sequence over the slab (tree.hip); the plan's ranges, row tile and workspace
+int tree_row_tile(const pplhip_tree_attention_args* a);
+int64_t tree_num_ranges(const pplhip_tree_attention_args* a, int cu_count);
+uint64_t tree_workspace_bytes(const pplhip_tree_attention_args* a, int64_t ranges);
+pplhip_retcode launch_tree_attention(const pplhip_tree_attention_args* a, int64_t ranges, void* ws, hipStream_t stream);
+pplhip_retcode launch_kv_score(const pplhip_kv_score_args* a, hipStream_t stream);
+// eviction and accepted drafts (evict.hip)
+uint64_t evict_workspace_bytes(const pplhip_kv_evict_args* a, int64_t max_moves);
+pplhip_retcode launch_kv_evict(const pplhip_kv_evict_args* a, int64_t max_moves, void* ws, hipStream_t stream);
+pplhip_retcode launch_kv_accept(const pplhip_kv_accept_args* a, hipStream_t stream);
 
 } // namespace pplhip
 

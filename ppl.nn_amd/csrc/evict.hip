@@ -1,0 +1,349 @@
+// Moves of cached rows inside the slab: eviction by accumulated attention weight, and keeping the accepted path of a
+// verified draft. Both are bound by the bytes of the rows they move; the choice of what to evict by reading the scores.
+//
+// Eviction. A sequence keeps K of its kvlen rows (per layer and kv head on its own). Only rows that stay but lie behind
+// the first K places move, each into the place of a row in front that goes: as few row moves as possible, and sources
+// (index >= K) and destinations (index < K) never overlap, so all of them run in parallel, in place.
+//
+// kv_evict_choose_kernel: one workgroup per (sequence, layer, kv head). The K-th largest key is found digit by digit (8
+// bits at a time, counts in LDS), then one more pass in index order numbers the holes and the rows that fill them.
+// kv_evict_move_kernel: 16-byte pieces of the listed rows, K and V, with their scales.
+#include "common.h"
+
+namespace pplhip {
+
+struct EvictParams {
+    const int64_t* kvstarts;
+    const int64_t* target;
+    const int64_t* next_pos;
+    PageMap pages;
+    CacheAddr addr; // layer: the first one
+    int8_t* cache;
+    half_t* scale;
+    const float* score_in;
+    float* score_out;
+    const int32_t* pos_in;
+    int32_t* pos_out;
+    int64_t score_stride_l, score_stride_h;
+    int64_t* new_kvlen;
+    int32_t num_sink, num_recent;
+    int32_t layer_count, kv_heads, pieces; // pieces: 16-byte pieces of a row
+    int32_t blocks_per_column;
+    int32_t max_moves;
+    int32_t* moves; // [columns]: rows to move
+    int32_t* holes; // [columns][max_moves]: index of the j-th hole ..
+    int32_t* fills; // .. and of the row that goes there
+};
+
+constexpr int kChooseThreads = 512;
+constexpr int kChooseWaves = kChooseThreads / 64;
+constexpr int kHistCopies = 16; // copies of the digit counts: scores share their leading bits, so lanes would queue
+
+struct EvictColumn {
+    int32_t b, layer, head;
+    int64_t scores; // offset of the column in the score and position arrays
+};
+__device__ inline EvictColumn evict_column(const EvictParams& p, int column) {
+    EvictColumn c;
+    c.head = column % p.kv_heads;
+    const int rest = column / p.kv_heads;
+    c.layer = rest % p.layer_count;
+    c.b = rest / p.layer_count;
+    c.scores = (int64_t)(p.addr.layer + c.layer) * p.score_stride_l + (int64_t)c.head * p.score_stride_h;
+    return c;
+}
+
+// Sort key of a token: larger stays. Protected tokens above everything, then the scores in their order, NaN lowest.
+__device__ inline uint32_t evict_key(const EvictParams& p, float score, int32_t pos, int64_t next) {
+    if (p.pos_in && (pos < p.num_sink || (p.num_recent > 0 && (int64_t)pos >= next - p.num_recent))) return 0xffffffffu;
+    if (score != score) return 0;
+    const uint32_t u = score == 0.f ? 0u : __float_as_uint(score); // (-0 counts as 0)
+    return u >> 31 ? ~u : u | 0x80000000u;
+}
+
+__global__ __launch_bounds__(kChooseThreads) void kv_evict_choose_kernel(const EvictParams p) {
+    __shared__ uint32_t hist[256 * kHistCopies];
+    __shared__ uint32_t wave_sum[kChooseWaves];
+    __shared__ uint32_t found[2]; // digit, rows above it
+    __shared__ int32_t seg_gt[kChooseWaves], seg_eq[kChooseWaves];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const EvictColumn col = evict_column(p, blockIdx.x);
+    const int64_t kvlen64 = p.kvstarts[col.b + 1] - p.kvstarts[col.b];
+    const int64_t want = p.target[col.b] < 0 ? 0 : p.target[col.b];
+    const int n = (int)kvlen64;
+    const int keep = want < kvlen64 ? (int)want : n;
+    const int64_t next = p.next_pos ? p.next_pos[col.b] : 0;
+    if (col.layer == 0 && col.head == 0 && tid == 0) p.new_kvlen[col.b] = keep;
+    const bool copy_score = p.score_out != p.score_in, copy_pos = p.pos_in && p.pos_out != p.pos_in;
+    if (keep == n || keep == 0) { // nothing moves
+        if (tid == 0) p.moves[blockIdx.x] = 0;
+        for (int j = tid; j < keep; j += kChooseThreads) {
+            const int64_t at = col.scores + p.pages.token(col.b, j);
+            if (copy_score) p.score_out[at] = p.score_in[at];
+            if (copy_pos) p.pos_out[at] = p.pos_in[at];
+        }
+        return;
+    }
+    auto key_of = [&](int j) {
+        const int64_t at = col.scores + p.pages.token(col.b, j);
+        return evict_key(p, p.score_in[at], p.pos_in ? p.pos_in[at] : 0, next);
+    };
+
+    // ---- the keep-th largest key: `prefix` collects its digits, `remain` counts rows still to be found below them
+    uint32_t prefix = 0;
+    uint32_t remain = (uint32_t)keep;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        for (int i = tid; i < 256 * kHistCopies; i += kChooseThreads) hist[i] = 0;
+        __syncthreads();
+        for (int j = tid; j < n; j += kChooseThreads) {
+            const uint32_t k = key_of(j);
+            if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8)))
+                atomicAdd(&hist[((k >> shift) & 255) * kHistCopies + (lane & (kHistCopies - 1))], 1u);
+        }
+        __syncthreads();
+        uint32_t mine = 0, incl = 0;
+        if (tid < 256) { // thread i: digit 255 - i, so that the running sum counts from the largest digit down
+            for (int c = 0; c < kHistCopies; ++c) mine += hist[(255 - tid) * kHistCopies + c];
+            incl = mine;
+            for (int d = 1; d < 64; d <<= 1) {
+                const uint32_t up = __shfl_up(incl, d);
+                if (lane >= d) incl += up;
+            }
+            if (lane == 63) wave_sum[wave] = incl;
+        }
+        __syncthreads();
+        if (tid < 256) {
+            for (int w = 0; w < wave; ++w) incl += wave_sum[w];
+            if (incl >= remain && incl - mine < remain) {
+                found[0] = 255 - tid;
+                found[1] = incl - mine;
+            }
+        }
+        __syncthreads();
+        prefix |= found[0] << shift;
+        remain -= found[1];
+        __syncthreads();
+    }
+    const int need_equal = (int)remain; // rows with exactly this key that stay: the first ones
+
+    // ---- in index order: every wave counts its own stretch, then numbers the rows in it
+    const int stretch = ((n + kChooseThreads - 1) / kChooseThreads) * 64;
+    const int j0 = wave * stretch, j1 = j0 + stretch < n ? j0 + stretch : n;
+    int gt = 0, eq = 0;
+    for (int j = j0; j < j1; j += 64) {
+        const bool in = j + lane < j1;
+        const uint32_t k = in ? key_of(j + lane) : 0;
+        gt += __popcll(__ballot(in && k > prefix));
+        eq += __popcll(__ballot(in && k == prefix));
+    }
+    if (lane == 0) {
+        seg_gt[wave] = gt;
+        seg_eq[wave] = eq;
+    }
+    __syncthreads();
+    int gt_before = 0, eq_before = 0;
+    for (int w = 0; w < wave; ++w) {
+        gt_before += seg_gt[w];
+        eq_before += seg_eq[w];
+    }
+    int32_t* const holes = p.holes + (int64_t)blockIdx.x * p.max_moves;
+    int32_t* const fills = p.fills + (int64_t)blockIdx.x * p.max_moves;
+    const uint64_t below = (uint64_t(1) << lane) - 1;
+    for (int j = j0; j < j1; j += 64) {
+        const int i = j + lane;
+        const bool in = i < j1;
+        const int64_t at = col.scores + p.pages.token(col.b, in ? i : j);
+        const float score = p.score_in[at];
+        const int32_t pos = p.pos_in ? p.pos_in[at] : 0;
+        const uint32_t k = evict_key(p, score, pos, next);
+        const uint64_t gts = __ballot(in && k > prefix), eqs = __ballot(in && k == prefix);
+        const int g0 = gt_before + __popcll(gts & below), e0 = eq_before + __popcll(eqs & below);
+        const int kept_before = g0 + (e0 < need_equal ? e0 : need_equal);
+        const bool stays = in && (k > prefix || (k == prefix && e0 < need_equal));
+        if (in && i < keep && !stays) holes[i - kept_before] = i;
+        if (stays && i >= keep) fills[keep - 1 - kept_before] = i;
+        if (stays && i < keep) {
+            if (copy_score) p.score_out[at] = score;
+            if (copy_pos) p.pos_out[at] = pos;
+        }
+        if (i == keep - 1) p.moves[blockIdx.x] = keep - kept_before - (stays ? 1 : 0);
+        gt_before += __popcll(gts);
+        eq_before += __popcll(eqs);
+    }
+}
+
+__global__ __launch_bounds__(256) void kv_evict_move_kernel(const EvictParams p) {
+    const int column = blockIdx.x / p.blocks_per_column;
+    const int block = blockIdx.x - column * p.blocks_per_column;
+    const int count = p.moves[column];
+    const EvictColumn col = evict_column(p, column);
+    const int32_t* const holes = p.holes + (int64_t)column * p.max_moves;
+    const int32_t* const fills = p.fills + (int64_t)column * p.max_moves;
+    CacheAddr addr = p.addr;
+    addr.layer += col.layer;
+    const int per_row = 2 * p.pieces;
+    const int64_t units = (int64_t)count * per_row;
+    for (int64_t u = (int64_t)block * 256 + threadIdx.x; u < units; u += (int64_t)p.blocks_per_column * 256) {
+        const int m = (int)(u / per_row);
+        const int r = (int)(u - (int64_t)m * per_row);
+        const int kv = r >= p.pieces, piece = r - kv * p.pieces;
+        const int64_t to = p.pages.token(col.b, holes[m]), from = p.pages.token(col.b, fills[m]);
+        const int64_t src = addr.row(from, kv, col.head) + 16 * piece, dst = addr.row(to, kv, col.head) + 16 * piece;
+        const uint4 q = *reinterpret_cast<const uint4*>(p.cache + src);
+        const uint32_t s = *reinterpret_cast<const uint32_t*>(p.scale + src / kQuantGroup);
+        *reinterpret_cast<uint4*>(p.cache + dst) = q;
+        *reinterpret_cast<uint32_t*>(p.scale + dst / kQuantGroup) = s;
+        if (r == 0) {
+            p.score_out[col.scores + to] = p.score_in[col.scores + from];
+            if (p.pos_in) p.pos_out[col.scores + to] = p.pos_in[col.scores + from];
+        }
+    }
+}
+
+int64_t evict_columns(const pplhip_kv_evict_args* a) {
+    return a->batch * a->layer_count * a->num_kv_heads;
+}
+uint64_t evict_workspace_bytes(const pplhip_kv_evict_args* a, int64_t max_moves) {
+    return (uint64_t)evict_columns(a) * (1 + 2 * (uint64_t)max_moves) * sizeof(int32_t);
+}
+
+pplhip_retcode launch_kv_evict(const pplhip_kv_evict_args* a, int64_t max_moves, void* ws, hipStream_t stream) {
+    EvictParams p;
+    p.kvstarts = a->d_kvstarts;
+    p.target = a->d_target_kvlen;
+    p.next_pos = a->num_recent > 0 ? a->d_next_pos : nullptr;
+    p.pages = PageMap{a->d_cachestarts, a->cachestart_stride_b, page_shift_of(a->cache_mode, a->page_size)};
+    p.addr = CacheAddr{a->cache_stride_s, a->cache_stride_l, a->cache_stride_h, a->cache_stride_kv, a->layer_idx};
+    p.cache = (int8_t*)a->d_cache;
+    p.scale = (half_t*)a->d_scale;
+    p.score_in = a->d_score_in;
+    p.score_out = a->d_score_out;
+    p.pos_in = a->d_position_in;
+    p.pos_out = a->d_position_out;
+    p.score_stride_l = a->score_stride_l;
+    p.score_stride_h = a->score_stride_h;
+    p.new_kvlen = a->d_new_kvlen;
+    p.num_sink = a->num_sink;
+    p.num_recent = a->num_recent;
+    p.layer_count = a->layer_count;
+    p.kv_heads = a->num_kv_heads;
+    p.pieces = a->head_dim / 16;
+    const int64_t columns = evict_columns(a);
+    p.max_moves = (int32_t)max_moves;
+    p.moves = (int32_t*)ws;
+    p.holes = p.moves + columns;
+    p.fills = p.holes + columns * max_moves;
+    hipLaunchKernelGGL(kv_evict_choose_kernel, dim3((unsigned)columns), dim3(kChooseThreads), 0, stream, p);
+    PPLHIP_CHECK_LAUNCH("kv_evict choose");
+    // how many rows move is known on the device only: enough workgroups to fill the chip a few times over, each of which
+    // walks its share of the column's list
+    const int64_t most = (max_moves * 2 * p.pieces + 255) / 256;
+    int64_t per_column = (8192 + columns - 1) / columns;
+    if (per_column > most) per_column = most;
+    if (per_column < 1) per_column = 1;
+    p.blocks_per_column = (int32_t)per_column;
+    if (max_moves > 0) {
+        hipLaunchKernelGGL(kv_evict_move_kernel, dim3((unsigned)(columns * per_column)), dim3(256), 0, stream, p);
+        PPLHIP_CHECK_LAUNCH("kv_evict move");
+    }
+    return PPLHIP_RC_SUCCESS;
+}
+
+// ---- accepted drafted tokens
+//
+// Row start + i becomes what row start + path[i] was; path is ascending, so path[i] >= i. A thread owns one 16-byte piece
+// of (layer, K or V, head) and takes the whole path through it, eight rows loaded before eight are stored: a stored
+// place (below 8 k + 8) is never a later batch's source (path[i] >= i >= 8 k + 8), and no other thread touches the piece.
+struct AcceptParams {
+    const int64_t* seqstarts;
+    const int64_t* start_pos;
+    const int64_t* accepted;
+    const int64_t* accepted_len;
+    int64_t accepted_stride_b, max_accepted;
+    PageMap pages;
+    CacheAddr addr;
+    int8_t* cache;
+    half_t* scale;
+    int32_t layer_count, kv_heads, pieces;
+    int32_t blocks_per_seq;
+};
+
+__global__ __launch_bounds__(256) void kv_accept_kernel(const AcceptParams p) {
+    constexpr int kRows = 8;
+    const int b = blockIdx.x / p.blocks_per_seq;
+    const int64_t unit = (int64_t)(blockIdx.x - b * p.blocks_per_seq) * 256 + threadIdx.x;
+    const int piece = (int)(unit % p.pieces);
+    const int64_t rest = unit / p.pieces;
+    const int head = (int)(rest % p.kv_heads);
+    const int64_t rest2 = rest / p.kv_heads;
+    const int kv = (int)(rest2 & 1);
+    const int64_t layer = rest2 >> 1;
+    if (layer >= p.layer_count) return;
+    CacheAddr addr = p.addr;
+    addr.layer += (int32_t)layer;
+    const int64_t drafted = p.seqstarts[b + 1] - p.seqstarts[b];
+    const int64_t start = p.start_pos[b];
+    const int64_t* const path = p.accepted + b * p.accepted_stride_b;
+    int64_t n = p.accepted_len[b];
+    if (n > p.max_accepted) n = p.max_accepted;
+    int64_t prev = -1;
+    for (int64_t i0 = 0; i0 < n; i0 += kRows) {
+        int64_t from[kRows];
+        uint4 q[kRows];
+        uint32_t s[kRows];
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) from[i] = i0 + i < n ? path[i0 + i] : -1;
+        int rows = 0; // entries of the batch before the list's end
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            if (rows == i && from[i] > prev && from[i] < drafted) {
+                prev = from[i];
+                rows = i + 1;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            if (i < rows && from[i] != i0 + i) {
+                const int64_t row = addr.row(p.pages.token(b, start + from[i]), kv, head) + 16 * piece;
+                q[i] = *reinterpret_cast<const uint4*>(p.cache + row);
+                s[i] = *reinterpret_cast<const uint32_t*>(p.scale + row / kQuantGroup);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            if (i < rows && from[i] != i0 + i) {
+                const int64_t row = addr.row(p.pages.token(b, start + i0 + i), kv, head) + 16 * piece;
+                *reinterpret_cast<uint4*>(p.cache + row) = q[i];
+                *reinterpret_cast<uint32_t*>(p.scale + row / kQuantGroup) = s[i];
+            }
+        }
+        if (rows < kRows) break;
+    }
+}
+
+pplhip_retcode launch_kv_accept(const pplhip_kv_accept_args* a, hipStream_t stream) {
+    AcceptParams p;
+    p.seqstarts = a->d_seqstarts;
+    p.start_pos = a->d_start_pos;
+    p.accepted = a->d_accepted;
+    p.accepted_len = a->d_accepted_len;
+    p.accepted_stride_b = a->accepted_stride_b;
+    p.max_accepted = a->max_accepted;
+    p.pages = PageMap{a->d_cachestarts, a->cachestart_stride_b, page_shift_of(a->cache_mode, a->page_size)};
+    p.addr = CacheAddr{a->cache_stride_s, a->cache_stride_l, a->cache_stride_h, a->cache_stride_kv, a->layer_idx};
+    p.cache = (int8_t*)a->d_cache;
+    p.scale = (half_t*)a->d_scale;
+    p.layer_count = a->layer_count;
+    p.kv_heads = a->num_kv_heads;
+    p.pieces = a->head_dim / 16;
+    const int64_t units = (int64_t)a->layer_count * 2 * a->num_kv_heads * p.pieces;
+    const int64_t per_seq = (units + 255) / 256;
+    if (per_seq * a->batch > 0x7fffffffLL) PPLHIP_FAIL(PPLHIP_RC_OUT_OF_RANGE, "kv_accept: too many rows");
+    p.blocks_per_seq = (int32_t)per_seq;
+    hipLaunchKernelGGL(kv_accept_kernel, dim3((unsigned)(per_seq * a->batch)), dim3(256), 0, stream, p);
+    PPLHIP_CHECK_LAUNCH("kv_accept");
+    return PPLHIP_RC_SUCCESS;
+}
+
+} // namespace pplhip
