@@ -50,6 +50,34 @@ __device__ inline void wave_lds_order() {
     __builtin_amdgcn_wave_barrier();
 }
 
+// The largest of four values held by lanes l, l ^ 16, l ^ 32, l ^ 48 (every lane gets it), and their sum: the swap
+// instructions hand every lane of a row pair both rows' values without a trip through LDS.
+__device__ inline float max_over_groups(float v) {
+    const uint32_t u = __float_as_uint(v);
+    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const uint32_t w = __float_as_uint(v);
+    const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ inline float sum_over_groups(float v) {
+    const uint32_t u = __float_as_uint(v);
+    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const uint32_t w = __float_as_uint(v);
+    const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// |int8| <= 128, and 128 * 511 is below fp16's largest: such a group's values are finite
+__device__ inline bool scale_is_small(half_t s) {
+    return __builtin_fabsf((float)s) < 511.f;
+}
+__device__ inline bool piece_is_small(uint32_t scales) { // of the two groups of a 16-byte piece
+    const half2_t s2 = as_half2(scales);
+    return scale_is_small(s2.x) && scale_is_small(s2.y);
+}
+
 template <int DH>
 struct CacheTile {
     static constexpr int PIECES = DH / 16; // 16-byte pieces of a row
@@ -95,17 +123,75 @@ struct CacheTile {
         }
     }
 
-    // bit r: row r may hold a value that is not finite (|int8| <= 128, and 128 * 511 is below fp16's largest)
+    // bit r: row r may hold a value that is not finite
     __device__ inline uint32_t odd_rows() const {
         uint32_t rows = 0;
 #pragma unroll
         for (int n = 0; n < NLD; ++n) {
-            const half2_t s2 = as_half2(s[n]);
-            const bool fine = __builtin_fabsf((float)s2.x) < 511.f && __builtin_fabsf((float)s2.y) < 511.f;
-            for (uint64_t bad = __ballot(!fine); bad; bad &= bad - 1)
+            for (uint64_t bad = __ballot(!piece_is_small(s[n])); bad; bad &= bad - 1)
                 rows |= 1u << ((__builtin_ctzll(bad) + 64 * n) / PIECES);
         }
         return rows;
+    }
+    // as stash, with zeros for the pieces that may hold such values
+    __device__ inline void stash_finite(half_t* tile) const {
+        CacheTile<DH> t = *this;
+#pragma unroll
+        for (int n = 0; n < NLD; ++n) t.s[n] = piece_is_small(s[n]) ? s[n] : 0u;
+        t.stash(tile);
+    }
+};
+
+// The same for a workgroup of W waves that shares the tile: a thread's pieces of the tile's K and V rows.
+template <int DH, int W>
+struct SharedTile {
+    static constexpr int PIECES = DH / 16;
+    static constexpr int ALL = 2 * kTileKeys * PIECES; // K's, then V's
+    static constexpr int NLD = (ALL + 64 * W - 1) / (64 * W);
+    static constexpr int LDR = DH + 8;
+    uint4_vt q[NLD];
+    uint32_t s[NLD];
+
+    // base: element offset of the tile's first K row
+    __device__ inline void fetch(const CacheView& v, int64_t base, int64_t kv0, int64_t kvlen) {
+        const int64_t n_left = kvlen - kv0;
+        const int last = n_left < kTileKeys ? (int)n_left - 1 : kTileKeys - 1;
+#pragma unroll
+        for (int n = 0; n < NLD; ++n) {
+            const int c = threadIdx.x + 64 * W * n;
+            const int kv = c >= kTileKeys * PIECES;
+            const int c2 = c - kv * kTileKeys * PIECES;
+            const int row = c2 / PIECES, piece = c2 - row * PIECES;
+            if (c < ALL && 16 * piece < v.head_dim) {
+                const int64_t off = base + (kv ? v.addr.stride_kv : 0) +
+                                    (int64_t)(row < last ? row : last) * v.addr.stride_s + 16 * piece;
+                q[n] = __builtin_nontemporal_load(reinterpret_cast<const uint4_vt*>(v.cache + off));
+                s[n] = *reinterpret_cast<const uint32_t*>((const char*)v.scale + off / 4);
+            } else {
+                q[n] = uint4_vt{0, 0, 0, 0};
+                s[n] = 0;
+            }
+        }
+    }
+    // odd: where to note the V rows with pieces that may not be finite (those become zeros); null: not looked at
+    __device__ inline void stash(half_t* k_tile, half_t* v_tile, uint32_t* odd) const {
+#pragma unroll
+        for (int n = 0; n < NLD; ++n) {
+            const int c = threadIdx.x + 64 * W * n;
+            if (ALL % (64 * W) != 0 && c >= ALL) break;
+            const int kv = c >= kTileKeys * PIECES;
+            const int c2 = c - kv * kTileKeys * PIECES;
+            const int row = c2 / PIECES, piece = c2 - row * PIECES;
+            uint32_t sc = s[n];
+            if (odd && kv && !piece_is_small(sc)) {
+                sc = 0;
+                atomicOr(odd, 1u << row);
+            }
+            const half2_t s2 = as_half2(sc);
+            half8_t* dst = reinterpret_cast<half8_t*>((kv ? v_tile : k_tile) + row * LDR + 16 * piece);
+            dst[0] = dequant8(q[n].x, q[n].y, s2.x);
+            dst[1] = dequant8(q[n].z, q[n].w, s2.y);
+        }
     }
 };
 

@@ -10,10 +10,14 @@
 //
 // Split. Work is laid out on one axis per kv head: for every sequence, for every row tile, its keys in tiles of 32. The
 // axis is cut into num_ranges equal ranges on the device (every workgroup sums the sequences' costs itself: no host
-// knowledge of the lengths, no planning launch); a workgroup walks the (sequence, row tile) pieces of its range, its four
-// waves taking every fourth key tile and combining in LDS at the end of a piece. A range can start and end inside a row
-// tile: such a piece leaves its partial in the workspace, at most two per range (the first and the last piece), and
-// tree_merge_kernel combines them.
+// knowledge of the lengths, no planning launch); a workgroup walks the (sequence, row tile) pieces of its range. A range
+// can start and end inside a row tile: such a piece leaves its partial in the workspace, at most two per range (the first
+// and the last piece), and tree_merge_kernel combines them.
+//
+// Two kernels share this. tree_keys_kernel (row tiles of 16 or 32 rows): every wave carries all rows and takes every
+// fourth key tile, through a region of LDS of its own; no barrier until the waves' shares are joined at the end of a
+// piece. tree_rows_kernel (64, 128 or 256 rows): the waves share out the rows and all read one key tile, which the whole
+// workgroup brings into LDS, so that a cached byte is dequantised once for all rows.
 #include "cache_tile.h"
 
 namespace pplhip {
@@ -39,12 +43,15 @@ struct TreeParams {
     int64_t* range_start; // [num_ranges][3]; sequence -1: nothing left for this range
 };
 
-constexpr int kTreeWaves = 4;
+constexpr int kTreeWaves = 4; // of tree_keys_kernel
 constexpr int64_t kPieceCost = 4; // what starting and finishing a row tile costs, in key tiles
 constexpr int64_t kMinRangeTiles = 8; // a range is at least this long: two key tiles per wave
-// Probabilities are held as 2^kProbShift * exp2(x - m): the fp16 operand of the second product then keeps full precision
-// for weights down to 2^-26 of the row's largest (2^-14 unshifted). Sums carry the same factor.
-constexpr float kProbShift = 12.f;
+// The reference point m of a row's exponents need not be its running maximum: it only moves when a score passes it by
+// more than 2^kSlack, so that most tiles need neither a maximum across lanes nor a rescaling. Weights are held as
+// exp2(x - m + kProbShift), at most 2^15 in fp16 (the operand of the second product); a weight keeps fp16's full
+// precision down to 2^-22 of 2^m. Sums carry the same factor and keep 32 bits.
+constexpr float kProbShift = 8.f;
+constexpr float kSlack = 7.f;
 
 __device__ inline int64_t uniform64(int64_t v) {
     const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v);
@@ -132,39 +139,212 @@ __device__ inline uint32_t visible_keys(const uint64_t* row_mask, int words, int
     return n >= 32 ? see : see & ((1u << n) - 1);
 }
 
-// NR: blocks of 16 rows a wave carries; the row tile has 16 * NR rows.
-template <int DH, int NR>
-__global__ __launch_bounds__(256, 2) void tree_attention_kernel(const TreeParams p) {
-    constexpr int ROWS = 16 * NR;
-    constexpr int LDR = CacheTile<DH>::LDR; // halves per LDS row
-    constexpr int LDO = DH + 4; // floats per row of the combination
-    constexpr int KC = DH / 16, KC2 = DH / 32;
-    static_assert(kTreeWaves * kTileKeys * LDR * 2 >= kTreeWaves * 16 * LDO * 4, "the combination reuses the tiles");
-    __shared__ __attribute__((aligned(16))) half_t lds[kTreeWaves * kTileKeys * LDR];
-    __shared__ float2 ml_lds[kTreeWaves][ROWS];
+// What a wave holds of its N blocks of 16 rows: lane (g = lane / 16, lane % 16) row lane % 16 of each block, of the output
+// channels 16 i + 4 g .. + 3 and of the sum its own keys' share.
+template <int DH, int N>
+struct RowState {
+    int64_t tok[N];
+    int head[N];
+    bool valid[N];
+    half8_t qf[N][DH / 32];
+    float m[N], shift[N], l[N]; // m in units of the raw products; shift = kProbShift - m * scale_log2
+    float4_t o[N][DH / 16];
 
-    const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int r_lane = lane & 15, g = lane >> 4;
-    const int hd = p.view.head_dim;
-    const int range = blockIdx.x / p.kv_heads;
-    const int kvh = blockIdx.x - range * p.kv_heads;
+    __device__ inline void start(const TreeParams& p, int64_t s0, int64_t rows, const int64_t (&first_row)[N], int kvh) {
+        const int lane = threadIdx.x & 63, g = lane >> 4;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int64_t row = first_row[n] + (lane & 15);
+            valid[n] = row < rows;
+            const int64_t rr = valid[n] ? row : rows - 1;
+            tok[n] = (uint64_t)rr >> 32 ? rr / p.rep : (int64_t)((uint32_t)rr / (uint32_t)p.rep);
+            head[n] = kvh * p.rep + (int)(rr - tok[n] * p.rep);
+            const half_t* qp = p.q + ((s0 + tok[n]) * p.num_heads + head[n]) * p.view.head_dim + 8 * g;
+#pragma unroll
+            for (int kc = 0; kc < DH / 32; ++kc) {
+                if (32 * kc + 8 * g < p.view.head_dim) {
+                    qf[n][kc] = *reinterpret_cast<const half8_t*>(qp + 32 * kc);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) qf[n][kc][e] = (half_t)0.f;
+                }
+            }
+            m[n] = -INFINITY;
+            shift[n] = kProbShift;
+            l[n] = 0.f;
+#pragma unroll
+            for (int i = 0; i < DH / 16; ++i) o[n][i] = float4_t{0.f, 0.f, 0.f, 0.f};
+        }
+    }
+
+    // scores of the rows against the 32 keys in `tile`: s[n][tb][e] belongs to key 16 * tb + 4 * g + e
+    __device__ inline void scores(const half_t* tile, float (&s)[N][2][4]) const {
+        const int lane = threadIdx.x & 63, g = lane >> 4;
+#pragma unroll
+        for (int tb = 0; tb < 2; ++tb) {
+            float4_t acc[N];
+#pragma unroll
+            for (int n = 0; n < N; ++n) acc[n] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int kc = 0; kc < DH / 32; ++kc) {
+                const half8_t a = *reinterpret_cast<const half8_t*>(tile + (16 * tb + (lane & 15)) * CacheTile<DH>::LDR +
+                                                                    32 * kc + 8 * g);
+#pragma unroll
+                for (int n = 0; n < N; ++n) acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qf[n][kc], acc[n], 0, 0, 0);
+            }
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[n][tb][e] = acc[n][e];
+        }
+    }
+
+    // keys a row does not see get score -inf; see[n]: bit i = key kv0 + i
+    __device__ inline void hide(const TreeParams& p, int64_t s0, int64_t kv0, int64_t start, int64_t kvlen,
+                                float (&s)[N][2][4], uint32_t (&see)[N]) const {
+        const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            see[n] = valid[n] ? visible_keys(p.mask ? p.mask + (s0 + tok[n]) * p.mask_words : nullptr, p.mask_words, tok[n],
+                                             kv0, start, kvlen)
+                              : 0u;
+            const uint32_t mine = see[n] >> (4 * g);
+#pragma unroll
+            for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[n][tb][e] = (mine >> (16 * tb + e)) & 1 ? s[n][tb][e] : -INFINITY;
+        }
+    }
+
+    // scores -> weights (left in s, and as fp16 in pp), running sums
+    __device__ inline void weights(float scale_log2, float (&s)[N][2][4], half8_t (&pp)[N]) {
+        float top[N];
+        bool moves = false;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            top[n] = fmaxf(fmaxf(fmaxf(s[n][0][0], s[n][0][1]), fmaxf(s[n][0][2], s[n][0][3])),
+                           fmaxf(fmaxf(s[n][1][0], s[n][1][1]), fmaxf(s[n][1][2], s[n][1][3])));
+            moves = moves || __builtin_fmaf(top[n], scale_log2, shift[n]) > kProbShift + kSlack ||
+                    (m[n] == -INFINITY && top[n] > -INFINITY);
+        }
+        if (__any(moves)) { // (rows without a key so far keep m = -inf: weights exp2(-inf) = 0)
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const float m_new = fmaxf(m[n], max_over_groups(top[n]));
+                const float ref = m_new == -INFINITY ? 0.f : m_new;
+                const float alpha = __builtin_amdgcn_exp2f((m[n] - ref) * scale_log2);
+                m[n] = m_new;
+                shift[n] = kProbShift - ref * scale_log2;
+                l[n] *= alpha;
+#pragma unroll
+                for (int i = 0; i < DH / 16; ++i) o[n][i] *= alpha;
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            float sum = 0.f;
+#pragma unroll
+            for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][tb][e], scale_log2, shift[n]));
+                    sum += w;
+                    s[n][tb][e] = w;
+                    pp[n][4 * tb + e] = (half_t)w;
+                }
+            l[n] += sum;
+        }
+    }
+
+    // o += weights x the 32 value rows in `tile`
+    __device__ inline void values(const half_t* tile, const half8_t (&pp)[N]) {
+        constexpr int LDR = CacheTile<DH>::LDR;
+        const int lane = threadIdx.x & 63, g = lane >> 4, j = lane & 15;
+#pragma unroll
+        for (int i = 0; i < DH / 16; ++i) {
+            // lane (g, j) receives channel 16 * i + j of keys 4 * g .. + 3 and 16 + 4 * g .. + 3
+            const half_t* src = tile + (4 * g + (j >> 2)) * LDR + 16 * i + 4 * (j & 3);
+            const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)src);
+            const short4_t hi =
+                __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)(src + 16 * LDR));
+            half8_t a;
+            __builtin_memcpy(&a, &lo, 8);
+            __builtin_memcpy(reinterpret_cast<char*>(&a) + 8, &hi, 8);
+#pragma unroll
+            for (int n = 0; n < N; ++n) o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pp[n], o[n][i], 0, 0, 0);
+        }
+    }
+
+    // Value pieces that may not be finite are zeros in the tile (a key can be hidden from a row: its weight there is 0,
+    // and 0 times a NaN or an infinity is NaN): they are added here, to the rows that see their key. rows: which rows of
+    // the tile have such pieces; base: element offset of its first V row.
+    __device__ inline void odd_values(const TreeParams& p, int64_t base, int64_t kv0, int64_t kvlen, uint32_t rows,
+                                      const float (&s)[N][2][4], const uint32_t (&see)[N]) {
+        const int lane = threadIdx.x & 63, g = lane >> 4;
+        for (; rows; rows &= rows - 1) {
+            const int row = __builtin_ctz(rows);
+            if (kv0 + row >= kvlen) break;
+            const int8_t* vq = p.view.cache + base + row * p.view.addr.stride_s;
+            const half_t* vs = p.view.scale + (base + row * p.view.addr.stride_s) / kQuantGroup;
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                float w = 0.f;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) w = (row & 3) + 4 * (row >> 4) == k ? s[n][k >> 2][k & 3] : w;
+                w = (float)(half_t)__shfl(w, 16 * ((row >> 2) & 3) + (lane & 15));
+                if (!((see[n] >> row) & 1)) continue;
+#pragma unroll
+                for (int i = 0; i < DH / 16; ++i) {
+                    if (16 * i >= p.view.head_dim || (scale_is_small(vs[2 * i]) && scale_is_small(vs[2 * i + 1]))) continue;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int d = 16 * i + 4 * g + e;
+                        o[n][i][e] += w * (float)(half_t)((float)vq[d] * (float)vs[d >> 3]);
+                    }
+                }
+            }
+        }
+    }
+};
+
+// Writes 4 channels of a finished row, and its log-sum with channel 0. l == 0: the row saw nothing (a NaN stays NaN).
+__device__ inline void finish_row(const TreeParams& p, int64_t s0, int64_t row, int kvh, int d, float4_t a, float m_log2,
+                                  float l) {
+    const int64_t t = row / p.rep;
+    const int64_t at = (s0 + t) * p.num_heads + kvh * p.rep + (row - t * p.rep);
+    const float inv = l != 0.f ? 1.0f / l : 0.f;
+    const half4_t r = {(half_t)(a[0] * inv), (half_t)(a[1] * inv), (half_t)(a[2] * inv), (half_t)(a[3] * inv)};
+    *reinterpret_cast<half4_t*>(p.out + at * p.view.head_dim + d) = r;
+    if (p.lse && d == 0) p.lse[at] = l == 0.f ? -INFINITY : (m_log2 + (log2f(l) - kProbShift)) * 0.693147180559945f;
+}
+
+// One (sequence, row tile) piece of a range, as far as both kernels agree on it.
+struct TreePiece {
+    int32_t b;
+    int64_t s0, start, kvlen, rows, row0; // row0: first row of the tile
+    int64_t key_tile, stop_tile; // key tiles to look at (causal rows see nothing past their own token)
+    bool whole; // all the row tile's keys are in this piece
+    int64_t slot; // else: where its partial goes
+};
+
+// Calls `piece` for every piece of workgroup (range, kvh)'s range.
+template <int ROWS, class F>
+__device__ inline void walk_range(const TreeParams& p, int range, int kvh, F&& piece) {
     const const_tab64_t seqstarts = (const_tab64_t)p.seqstarts, kvstarts = (const_tab64_t)p.kvstarts;
-    half_t* const tile = lds + wave * kTileKeys * LDR;
-
     const RangeStart rs = find_range(p, range, ROWS);
     int64_t left = rs.length;
     int b = rs.b;
     int64_t row_tile = rs.row_tile, key_tile = rs.key_tile;
     int64_t first_b = -1, first_row_tile = 0, first_key_tile = 0;
-    bool first_piece = true;
     while (left > 0 && b < p.batch) {
-        const int64_t s0 = seqstarts[b];
-        const int64_t L = seqstarts[b + 1] - s0;
-        const int64_t kvlen = kvstarts[b + 1] - kvstarts[b];
-        const int64_t rows = L * p.rep;
-        const int64_t row_tiles = L <= 0 ? 0 : (rows + ROWS - 1) / ROWS;
-        const int64_t key_tiles = (kvlen + kTileKeys - 1) / kTileKeys;
+        TreePiece t;
+        t.b = b;
+        t.s0 = seqstarts[b];
+        const int64_t L = seqstarts[b + 1] - t.s0;
+        t.kvlen = kvstarts[b + 1] - kvstarts[b];
+        t.rows = L * p.rep;
+        const int64_t row_tiles = L <= 0 ? 0 : (t.rows + ROWS - 1) / ROWS;
+        const int64_t key_tiles = (t.kvlen + kTileKeys - 1) / kTileKeys;
         if (row_tile >= row_tiles) {
             ++b;
             row_tile = key_tile = 0;
@@ -172,261 +352,25 @@ __global__ __launch_bounds__(256, 2) void tree_attention_kernel(const TreeParams
         }
         const int64_t end_tile = key_tile + left < key_tiles ? key_tile + left : key_tiles;
         if (key_tile < end_tile) {
-            if (first_piece) {
+            if (first_b < 0) {
                 first_b = b;
                 first_row_tile = row_tile;
                 first_key_tile = key_tile;
             }
-            const int64_t start = kvlen - L;
-            const int64_t row0 = row_tile * ROWS;
-            // causal rows see nothing past the tile's last token
-            const int64_t last_row = row0 + ROWS < rows ? row0 + ROWS - 1 : rows - 1;
-            int64_t stop_tile = end_tile;
+            t.start = t.kvlen - L;
+            t.row0 = row_tile * ROWS;
+            t.key_tile = key_tile;
+            t.stop_tile = end_tile;
             if (!p.mask) {
-                const int64_t t = (start + last_row / p.rep + kTileKeys) / kTileKeys;
-                stop_tile = t < stop_tile ? t : stop_tile;
+                const int64_t last_row = t.row0 + ROWS < t.rows ? t.row0 + ROWS - 1 : t.rows - 1;
+                const int64_t last = (t.start + last_row / p.rep + kTileKeys) / kTileKeys;
+                t.stop_tile = last < end_tile ? last : end_tile;
             }
-            int64_t tok[NR];
-            int head[NR];
-            bool valid[NR];
-            half8_t qf[NR][KC2];
-#pragma unroll
-            for (int n = 0; n < NR; ++n) {
-                const int64_t row = row0 + 16 * n + r_lane;
-                valid[n] = row < rows;
-                const int64_t rr = valid[n] ? row : rows - 1;
-                tok[n] = rr / p.rep;
-                head[n] = kvh * p.rep + (int)(rr - tok[n] * p.rep);
-                const half_t* qp = p.q + ((s0 + tok[n]) * p.num_heads + head[n]) * hd + 8 * g;
-#pragma unroll
-                for (int kc = 0; kc < KC2; ++kc) {
-                    if (32 * kc + 8 * g < hd) {
-                        qf[n][kc] = *reinterpret_cast<const half8_t*>(qp + 32 * kc);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) qf[n][kc][e] = (half_t)0.f;
-                    }
-                }
-            }
-            float m_run[NR], l_run[NR];
-            float4_t o[NR][KC];
-#pragma unroll
-            for (int n = 0; n < NR; ++n) {
-                m_run[n] = -INFINITY;
-                l_run[n] = 0.f;
-#pragma unroll
-                for (int i = 0; i < KC; ++i) o[n][i] = float4_t{0.f, 0.f, 0.f, 0.f};
-            }
-
-            CacheTile<DH> rk, rv;
-            int64_t kt = key_tile + wave;
-            int64_t base = 0;
-            if (kt < stop_tile) {
-                base = p.view.key_row(b, kt * kTileKeys, kvh);
-                rk.fetch(p.view, base, kt * kTileKeys, kvlen);
-                rv.fetch(p.view, base + p.view.addr.stride_kv, kt * kTileKeys, kvlen);
-            }
-            for (; kt < stop_tile; kt += kTreeWaves) {
-                const int64_t kv0 = kt * kTileKeys;
-                const bool more = kt + kTreeWaves < stop_tile;
-                wave_lds_order();
-                rk.stash(tile);
-                wave_lds_order();
-                if (more) {
-                    base = p.view.key_row(b, kv0 + kTreeWaves * kTileKeys, kvh);
-                    rk.fetch(p.view, base, kv0 + kTreeWaves * kTileKeys, kvlen);
-                }
-                // ---- scores: lane (g, r_lane) gets rows' column r_lane, keys 16 * tb + 4 * g + e
-                float s[NR][2][4];
-#pragma unroll
-                for (int tb = 0; tb < 2; ++tb) {
-                    float4_t acc[NR];
-#pragma unroll
-                    for (int n = 0; n < NR; ++n) acc[n] = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int kc = 0; kc < KC2; ++kc) {
-                        const half8_t a = *reinterpret_cast<const half8_t*>(tile + (16 * tb + r_lane) * LDR + 32 * kc + 8 * g);
-#pragma unroll
-                        for (int n = 0; n < NR; ++n)
-                            acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qf[n][kc], acc[n], 0, 0, 0);
-                    }
-#pragma unroll
-                    for (int n = 0; n < NR; ++n)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) s[n][tb][e] = acc[n][e];
-                }
-                const bool history = kv0 + kTileKeys <= start; // every row sees every key
-                uint32_t see[NR];
-                if (!history) {
-#pragma unroll
-                    for (int n = 0; n < NR; ++n) {
-                        see[n] = valid[n] ? visible_keys(p.mask ? p.mask + (s0 + tok[n]) * p.mask_words : nullptr,
-                                                         p.mask_words, tok[n], kv0, start, kvlen)
-                                          : 0u;
-#pragma unroll
-                        for (int tb = 0; tb < 2; ++tb)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                s[n][tb][e] = (see[n] >> (16 * tb + 4 * g + e)) & 1 ? s[n][tb][e] : -INFINITY;
-                    }
-                }
-                // ---- running maximum, probabilities, sum
-                half8_t pp[NR];
-                float alpha[NR];
-                bool still = true;
-#pragma unroll
-                for (int n = 0; n < NR; ++n) {
-                    float m = s[n][0][0];
-#pragma unroll
-                    for (int tb = 0; tb < 2; ++tb)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) m = fmaxf(m, s[n][tb][e]);
-                    m = fmaxf(m, __shfl_xor(m, 16));
-                    m = fmaxf(m, __shfl_xor(m, 32));
-                    const float m_new = fmaxf(m_run[n], m);
-                    // a row that has seen nothing yet: probabilities exp2(-inf) = 0, not NaN
-                    const float m_safe = m_new == -INFINITY ? 0.f : m_new;
-                    alpha[n] = __builtin_amdgcn_exp2f((m_run[n] - m_safe) * p.scale_log2);
-                    const float shift = kProbShift - m_safe * p.scale_log2;
-                    float sum = 0.f;
-#pragma unroll
-                    for (int tb = 0; tb < 2; ++tb)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][tb][e], p.scale_log2, shift));
-                            sum += pr;
-                            s[n][tb][e] = pr;
-                            pp[n][4 * tb + e] = (half_t)pr; // fp16 for the matrix product; the sum keeps 32 bits
-                        }
-                    l_run[n] = l_run[n] * alpha[n] + sum; // the lane's share: its own 8 keys of every tile
-                    m_run[n] = m_new;
-                    still = still && alpha[n] == 1.0f;
-                }
-                if (!__all(still)) {
-#pragma unroll
-                    for (int n = 0; n < NR; ++n)
-#pragma unroll
-                        for (int i = 0; i < KC; ++i) o[n][i] *= alpha[n];
-                }
-                // ---- values. Among the new tokens a key may be hidden from some rows; its weight there is 0, and 0 times
-                // a NaN or an infinity is NaN: such value rows are kept out of the matrix product and added row by row.
-                const uint32_t odd_rows = history ? 0u : rv.odd_rows();
-                wave_lds_order();
-                rv.stash(tile);
-                wave_lds_order();
-                if (odd_rows) {
-                    for (uint32_t rest = odd_rows; rest; rest &= rest - 1) {
-                        const int row = __builtin_ctz(rest);
-                        if (lane < DH / 16) {
-                            const uint4_vt z{0, 0, 0, 0};
-                            uint4_vt* dst = reinterpret_cast<uint4_vt*>(tile + row * LDR + 16 * lane);
-                            dst[0] = z;
-                            dst[1] = z;
-                        }
-                    }
-                    wave_lds_order();
-                }
-                if (more) rv.fetch(p.view, base + p.view.addr.stride_kv, kv0 + kTreeWaves * kTileKeys, kvlen);
-#pragma unroll
-                for (int i = 0; i < KC; ++i) {
-                    // lane (g, j) receives channel 16 * i + j of keys 4 * g .. + 3 and 16 + 4 * g .. + 3
-                    const half_t* src = tile + (4 * g + (r_lane >> 2)) * LDR + 16 * i + 4 * (r_lane & 3);
-                    const short4_t lo =
-                        __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)src);
-                    const short4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (__attribute__((address_space(3))) short4_t*)(src + 16 * LDR));
-                    half8_t a;
-                    __builtin_memcpy(&a, &lo, 8);
-                    __builtin_memcpy(reinterpret_cast<char*>(&a) + 8, &hi, 8);
-#pragma unroll
-                    for (int n = 0; n < NR; ++n) o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pp[n], o[n][i], 0, 0, 0);
-                }
-                if (odd_rows) {
-                    const int64_t vbase = p.view.key_row(b, kv0, kvh) + p.view.addr.stride_kv;
-                    for (uint32_t rest = odd_rows; rest; rest &= rest - 1) {
-                        const int row = __builtin_ctz(rest);
-                        if (kv0 + row >= kvlen) break;
-                        const int8_t* vq = p.view.cache + vbase + row * p.view.addr.stride_s;
-                        const half_t* vs = p.view.scale + (vbase + row * p.view.addr.stride_s) / kQuantGroup;
-#pragma unroll
-                        for (int n = 0; n < NR; ++n) {
-                            float w = 0.f;
-#pragma unroll
-                            for (int k = 0; k < 8; ++k) w = (row & 3) + 4 * (row >> 4) == k ? s[n][k >> 2][k & 3] : w;
-                            w = (float)(half_t)__shfl(w, 16 * ((row >> 2) & 3) + r_lane);
-                            if ((see[n] >> row) & 1) {
-#pragma unroll
-                                for (int i = 0; i < KC; ++i)
-#pragma unroll
-                                    for (int e = 0; e < 4; ++e) {
-                                        const int d = 16 * i + 4 * g + e;
-                                        if (d < hd) o[n][i][e] += w * (float)(half_t)((float)vq[d] * (float)vs[d >> 3]);
-                                    }
-                            }
-                        }
-                    }
-                }
-            }
-
-            // ---- the four waves' shares of the piece, combined 16 rows at a time
-            const bool whole = key_tile == 0 && end_tile == key_tiles;
-            const int64_t slot = 2 * (int64_t)range + (key_tile == 0 ? 1 : 0);
-            __syncthreads(); // (the tiles are read no more; the piece before has been written out)
-#pragma unroll
-            for (int n = 0; n < NR; ++n) {
-                l_run[n] += __shfl_xor(l_run[n], 16);
-                l_run[n] += __shfl_xor(l_run[n], 32);
-                if (g == 0) ml_lds[wave][16 * n + r_lane] = make_float2(m_run[n] * p.scale_log2, l_run[n]);
-            }
-            __syncthreads();
-            float* const olds = reinterpret_cast<float*>(lds);
-#pragma unroll
-            for (int n = 0; n < NR; ++n) {
-                float m = -INFINITY;
-                for (int w = 0; w < kTreeWaves; ++w) m = fmaxf(m, ml_lds[w][16 * n + r_lane].x);
-                const float m_safe = m == -INFINITY ? 0.f : m;
-                const float f = __builtin_amdgcn_exp2f(m_run[n] * p.scale_log2 - m_safe);
-                if (n) __syncthreads();
-#pragma unroll
-                for (int i = 0; i < KC; ++i)
-                    *reinterpret_cast<float4_t*>(olds + (wave * 16 + r_lane) * LDO + 16 * i + 4 * g) = o[n][i] * f;
-                __syncthreads();
-                for (int x = threadIdx.x; x < 16 * (DH / 4); x += 256) {
-                    const int r = x / (DH / 4), d = (x - r * (DH / 4)) * 4;
-                    float mm = -INFINITY;
-                    for (int w = 0; w < kTreeWaves; ++w) mm = fmaxf(mm, ml_lds[w][16 * n + r].x);
-                    const float mm_safe = mm == -INFINITY ? 0.f : mm;
-                    float l = 0.f;
-                    float4_t a = {0.f, 0.f, 0.f, 0.f};
-                    for (int w = 0; w < kTreeWaves; ++w) {
-                        const float2 ml = ml_lds[w][16 * n + r];
-                        l += ml.y * __builtin_amdgcn_exp2f(ml.x - mm_safe);
-                        a += *reinterpret_cast<const float4_t*>(olds + (w * 16 + r) * LDO + d);
-                    }
-                    const int64_t row = row0 + 16 * n + r;
-                    if (whole) {
-                        if (row < rows && d < hd) {
-                            const int64_t t = row / p.rep;
-                            const int64_t at = (s0 + t) * p.num_heads + kvh * p.rep + (row - t * p.rep);
-                            const float inv = l != 0.f ? 1.0f / l : 0.f; // (NaN stays NaN)
-                            const half4_t r4 = {(half_t)(a[0] * inv), (half_t)(a[1] * inv), (half_t)(a[2] * inv),
-                                                (half_t)(a[3] * inv)};
-                            *reinterpret_cast<half4_t*>(p.out + at * hd + d) = r4;
-                            if (p.lse && d == 0)
-                                p.lse[at] = l == 0.f ? -INFINITY : (mm + (log2f(l) - kProbShift)) * 0.693147180559945f;
-                        }
-                    } else {
-                        const int64_t at = ((int64_t)kvh * 2 * p.num_ranges + slot) * ROWS + 16 * n + r;
-                        *reinterpret_cast<float4_t*>(p.part_o + at * DH + d) = a;
-                        if (d == 0) p.part_ml[at] = make_float2(mm, l);
-                    }
-                }
-            }
-            __syncthreads();
-            first_piece = false;
+            t.whole = key_tile == 0 && end_tile == key_tiles;
+            t.slot = (int64_t)kvh * 2 * p.num_ranges + 2 * (int64_t)range + (key_tile == 0 ? 1 : 0);
+            piece(t);
         }
-        const int64_t to_next = key_tiles + kPieceCost - key_tile;
-        left -= to_next;
+        left -= key_tiles + kPieceCost - key_tile;
         ++row_tile;
         key_tile = 0;
     }
@@ -437,11 +381,207 @@ __global__ __launch_bounds__(256, 2) void tree_attention_kernel(const TreeParams
     }
 }
 
+// What the register allocator is to leave room for: above head_dim 128 two row blocks need more than half a SIMD's registers.
+constexpr int tree_waves_per_simd(int dh, int row_blocks) {
+    return dh > 128 && row_blocks > 1 ? 1 : 2;
+}
+
+// NR: blocks of 16 rows every wave carries; the row tile has 16 * NR rows.
+template <int DH, int NR>
+__global__ __launch_bounds__(256, tree_waves_per_simd(DH, NR)) void tree_keys_kernel(const TreeParams p) {
+    constexpr int ROWS = 16 * NR;
+    constexpr int LDR = CacheTile<DH>::LDR;
+    constexpr int LDO = DH + 4; // floats per row of the combination
+    static_assert(kTreeWaves * kTileKeys * LDR * 2 >= kTreeWaves * 16 * LDO * 4, "the combination reuses the tiles");
+    __shared__ __attribute__((aligned(16))) half_t lds[kTreeWaves * kTileKeys * LDR];
+    __shared__ float2 ml_lds[kTreeWaves][ROWS];
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r_lane = lane & 15, g = lane >> 4;
+    const int range = blockIdx.x / p.kv_heads;
+    const int kvh = blockIdx.x - range * p.kv_heads;
+    half_t* const tile = lds + wave * kTileKeys * LDR;
+
+    walk_range<ROWS>(p, range, kvh, [&](const TreePiece& t) {
+        RowState<DH, NR> st;
+        int64_t first_row[NR];
+#pragma unroll
+        for (int n = 0; n < NR; ++n) first_row[n] = t.row0 + 16 * n;
+        st.start(p, t.s0, t.rows, first_row, kvh);
+
+        CacheTile<DH> rk, rv; // the next tile's K and V rows, on their way
+        int64_t kt = t.key_tile + wave;
+        int64_t base = 0, base_now = 0;
+        if (kt < t.stop_tile) {
+            base = p.view.key_row(t.b, kt * kTileKeys, kvh);
+            rk.fetch(p.view, base, kt * kTileKeys, t.kvlen);
+            rv.fetch(p.view, base + p.view.addr.stride_kv, kt * kTileKeys, t.kvlen);
+        }
+        for (; kt < t.stop_tile; kt += kTreeWaves) {
+            const int64_t kv0 = kt * kTileKeys, kv_next = kv0 + kTreeWaves * kTileKeys;
+            const bool more = kt + kTreeWaves < t.stop_tile;
+            const bool history = kv0 + kTileKeys <= t.start; // every row sees every key
+            base_now = base;
+            wave_lds_order();
+            rk.stash(tile);
+            wave_lds_order();
+            if (more) {
+                base = p.view.key_row(t.b, kv_next, kvh);
+                rk.fetch(p.view, base, kv_next, t.kvlen);
+            }
+            float s[NR][2][4];
+            uint32_t see[NR];
+            half8_t pp[NR];
+            st.scores(tile, s);
+            if (!history) st.hide(p, t.s0, kv0, t.start, t.kvlen, s, see);
+            st.weights(p.scale_log2, s, pp);
+            const uint32_t odd = history ? 0u : rv.odd_rows();
+            wave_lds_order();
+            if (odd)
+                rv.stash_finite(tile);
+            else
+                rv.stash(tile);
+            wave_lds_order();
+            if (more) rv.fetch(p.view, base + p.view.addr.stride_kv, kv_next, t.kvlen);
+            st.values(tile, pp);
+            if (odd) st.odd_values(p, base_now + p.view.addr.stride_kv, kv0, t.kvlen, odd, s, see);
+        }
+
+        // ---- the four waves' shares of the piece, joined 16 rows at a time
+        __syncthreads(); // (the tiles are read no more; the piece before has been written out)
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+            const float l = sum_over_groups(st.l[n]);
+            if (g == 0) ml_lds[wave][16 * n + r_lane] = make_float2(st.m[n] * p.scale_log2, l);
+        }
+        __syncthreads();
+        float* const olds = reinterpret_cast<float*>(lds);
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+            float m = -INFINITY;
+            for (int w = 0; w < kTreeWaves; ++w) m = fmaxf(m, ml_lds[w][16 * n + r_lane].x);
+            const float f = __builtin_amdgcn_exp2f(st.m[n] * p.scale_log2 - (m == -INFINITY ? 0.f : m));
+            if (n) __syncthreads();
+#pragma unroll
+            for (int i = 0; i < DH / 16; ++i)
+                *reinterpret_cast<float4_t*>(olds + (wave * 16 + r_lane) * LDO + 16 * i + 4 * g) = st.o[n][i] * f;
+            __syncthreads();
+            for (int x = threadIdx.x; x < 16 * (DH / 4); x += 256) {
+                const int r = x / (DH / 4), d = (x - r * (DH / 4)) * 4;
+                float mm = -INFINITY;
+                for (int w = 0; w < kTreeWaves; ++w) mm = fmaxf(mm, ml_lds[w][16 * n + r].x);
+                float l = 0.f;
+                float4_t a = {0.f, 0.f, 0.f, 0.f};
+                for (int w = 0; w < kTreeWaves; ++w) {
+                    const float2 ml = ml_lds[w][16 * n + r];
+                    l += ml.y * __builtin_amdgcn_exp2f(ml.x - (mm == -INFINITY ? 0.f : mm));
+                    a += *reinterpret_cast<const float4_t*>(olds + (w * 16 + r) * LDO + d);
+                }
+                const int64_t row = t.row0 + 16 * n + r;
+                if (t.whole) {
+                    if (row < t.rows && d < p.view.head_dim) finish_row(p, t.s0, row, kvh, d, a, mm, l);
+                } else {
+                    const int64_t at = t.slot * ROWS + 16 * n + r;
+                    *reinterpret_cast<float4_t*>(p.part_o + at * DH + d) = a;
+                    if (d == 0) p.part_ml[at] = make_float2(mm, l);
+                }
+            }
+        }
+        __syncthreads();
+    });
+}
+
+// W waves, each with NB blocks of 16 rows: row block i of the tile is block i / W of wave i % W, so that few rows still
+// spread over all waves. The workgroup's threads bring a key tile's K and V pieces into one of two LDS buffers while the
+// other is computed on: one barrier per tile.
+template <int DH, int W, int NB>
+__global__ __launch_bounds__(W * 64, tree_waves_per_simd(DH, NB)) void tree_rows_kernel(const TreeParams p) {
+    constexpr int ROWS = 16 * W * NB;
+    constexpr int LDR = CacheTile<DH>::LDR;
+    __shared__ __attribute__((aligned(16))) half_t lds[2][2][kTileKeys * LDR]; // [buffer][K, V]
+    __shared__ uint32_t odd_lds[3]; // tile i's value rows that were kept out, in entry i % 3
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4;
+    const int range = blockIdx.x / p.kv_heads;
+    const int kvh = blockIdx.x - range * p.kv_heads;
+
+    walk_range<ROWS>(p, range, kvh, [&](const TreePiece& t) {
+        RowState<DH, NB> st;
+        int64_t first_row[NB];
+#pragma unroll
+        for (int n = 0; n < NB; ++n) first_row[n] = t.row0 + 16 * (wave + W * n);
+        st.start(p, t.s0, t.rows, first_row, kvh);
+        const bool busy = first_row[0] < t.rows; // (a wave without rows only helps to bring the tiles)
+        const int n_tiles = (int)(t.stop_tile - t.key_tile);
+
+        SharedTile<DH, W> raw[2]; // tiles i + 1 and i + 2, on their way
+        auto fetch = [&](SharedTile<DH, W>& r, int i) {
+            const int64_t kv0 = (t.key_tile + i) * kTileKeys;
+            r.fetch(p.view, p.view.key_row(t.b, kv0, kvh), kv0, t.kvlen);
+        };
+        auto stash = [&](const SharedTile<DH, W>& r, int i) {
+            const bool history = (t.key_tile + i + 1) * kTileKeys <= t.start;
+            r.stash(lds[i & 1][0], lds[i & 1][1], history ? nullptr : &odd_lds[i % 3]);
+        };
+        __syncthreads(); // (the piece before has read its last tile)
+        if (threadIdx.x < 3) odd_lds[threadIdx.x] = 0;
+        if (n_tiles > 0) fetch(raw[0], 0);
+        if (n_tiles > 1) fetch(raw[1], 1);
+        __syncthreads();
+        if (n_tiles > 0) stash(raw[0], 0);
+        if (n_tiles > 2) fetch(raw[0], 2);
+        __syncthreads();
+        auto step = [&](SharedTile<DH, W>& next, int i) { // next: tile i + 1, then tile i + 3
+            if (threadIdx.x == 0) odd_lds[(i + 2) % 3] = 0;
+            if (busy) {
+                const int64_t kv0 = (t.key_tile + i) * kTileKeys;
+                const bool history = kv0 + kTileKeys <= t.start;
+                float s[NB][2][4];
+                uint32_t see[NB];
+                half8_t pp[NB];
+                st.scores(lds[i & 1][0], s);
+                if (!history) st.hide(p, t.s0, kv0, t.start, t.kvlen, s, see);
+                st.weights(p.scale_log2, s, pp);
+                st.values(lds[i & 1][1], pp);
+                const uint32_t odd = history ? 0u : __builtin_amdgcn_readfirstlane(odd_lds[i % 3]);
+                if (odd)
+                    st.odd_values(p, p.view.key_row(t.b, kv0, kvh) + p.view.addr.stride_kv, kv0, t.kvlen, odd, s, see);
+            }
+            if (i + 1 < n_tiles) stash(next, i + 1);
+            if (i + 3 < n_tiles) fetch(next, i + 3);
+            __syncthreads();
+        };
+        for (int i = 0; i < n_tiles; i += 2) {
+            step(raw[1], i);
+            if (i + 1 < n_tiles) step(raw[0], i + 1);
+        }
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            const float l = sum_over_groups(st.l[n]);
+            const int r = 16 * (wave + W * n) + (lane & 15); // within the tile
+            if (t.whole) {
+#pragma unroll
+                for (int i = 0; i < DH / 16; ++i)
+                    if (st.valid[n] && 16 * i < p.view.head_dim)
+                        finish_row(p, t.s0, t.row0 + r, kvh, 16 * i + 4 * g, st.o[n][i], st.m[n] * p.scale_log2, l);
+            } else if (st.valid[n]) {
+                const int64_t at = t.slot * ROWS + r;
+#pragma unroll
+                for (int i = 0; i < DH / 16; ++i)
+                    *reinterpret_cast<float4_t*>(p.part_o + at * DH + 16 * i + 4 * g) = st.o[n][i];
+                if (g == 0) p.part_ml[at] = make_float2(st.m[n] * p.scale_log2, l);
+            }
+        }
+    });
+}
+
 // One workgroup per (range boundary, kv head): if the boundary is the first one inside its row tile, combines the row
 // tile's partials: the last piece of the range before it, then the first pieces of the ranges behind it.
-template <int DH, int NR>
-__global__ __launch_bounds__(256) void tree_merge_kernel(const TreeParams p) {
-    constexpr int ROWS = 16 * NR;
+template <int DH>
+__global__ __launch_bounds__(256) void tree_merge_kernel(const TreeParams p, const int ROWS) {
     const int range = 1 + blockIdx.x / p.kv_heads;
     const int kvh = blockIdx.x % p.kv_heads;
     const const_tab64_t st = (const_tab64_t)p.range_start;
@@ -471,23 +611,19 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeParams p) {
             a = a * fo + v * fn;
             m = m_new;
         }
-        const int64_t t = row / p.rep;
-        const int64_t at = (s0 + t) * p.num_heads + kvh * p.rep + (row - t * p.rep);
-        const float inv = l != 0.f ? 1.0f / l : 0.f;
-        const half4_t r4 = {(half_t)(a[0] * inv), (half_t)(a[1] * inv), (half_t)(a[2] * inv), (half_t)(a[3] * inv)};
-        *reinterpret_cast<half4_t*>(p.out + at * p.view.head_dim + d) = r4;
-        if (p.lse && d == 0) p.lse[at] = l == 0.f ? -INFINITY : (m + (log2f(l) - kProbShift)) * 0.693147180559945f;
+        finish_row(p, s0, row, kvh, d, a, m, l);
     }
 }
 
 // ---- host side
 
-static int tree_row_blocks(const pplhip_tree_attention_args* a) {
-    return a->max_seqlen * (a->num_heads / a->num_kv_heads) <= 16 ? 1 : 2;
-}
+// Rows of the longest sequence's (token, shared head) pairs decide the row tile: the smallest that holds them, 256 at
+// most (128 above head_dim 128, where two row blocks' accumulators leave no room for a third wave's worth of registers).
 int tree_row_tile(const pplhip_tree_attention_args* a) {
-    return 16 * tree_row_blocks(a);
+    const int64_t rows = a->max_seqlen * (a->num_heads / a->num_kv_heads);
+    return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 || a->head_dim > 128 ? 128 : 256;
 }
+
 // As many ranges as workgroups are resident (two per CU), shared out among the kv heads; never more than ranges of the
 // least length in the longest possible axis.
 int64_t tree_num_ranges(const pplhip_tree_attention_args* a, int cu_count) {
@@ -506,15 +642,20 @@ uint64_t tree_workspace_bytes(const pplhip_tree_attention_args* a, int64_t range
 }
 
 template <int DH>
-static void launch_tree_dh(const TreeParams& p, int nr, hipStream_t stream) {
+static void launch_tree_dh(const TreeParams& p, int row_tile, hipStream_t stream) {
     const dim3 grid((unsigned)(p.num_ranges * p.kv_heads));
-    const dim3 mgrid((unsigned)((p.num_ranges - 1) * p.kv_heads), (unsigned)(16 * nr * (DH / 4) / 256 > 0 ? 16 * nr * (DH / 4) / 256 : 1));
-    if (nr == 1) {
-        hipLaunchKernelGGL((tree_attention_kernel<DH, 1>), grid, dim3(256), 0, stream, p);
-        if (p.num_ranges > 1) hipLaunchKernelGGL((tree_merge_kernel<DH, 1>), mgrid, dim3(256), 0, stream, p);
-    } else {
-        hipLaunchKernelGGL((tree_attention_kernel<DH, 2>), grid, dim3(256), 0, stream, p);
-        if (p.num_ranges > 1) hipLaunchKernelGGL((tree_merge_kernel<DH, 2>), mgrid, dim3(256), 0, stream, p);
+    switch (row_tile) {
+        case 16: hipLaunchKernelGGL((tree_keys_kernel<DH, 1>), grid, dim3(256), 0, stream, p); break;
+        case 32: hipLaunchKernelGGL((tree_keys_kernel<DH, 2>), grid, dim3(256), 0, stream, p); break;
+        case 64: hipLaunchKernelGGL((tree_rows_kernel<DH, 4, 1>), grid, dim3(256), 0, stream, p); break;
+        case 128: hipLaunchKernelGGL((tree_rows_kernel<DH, 4, 2>), grid, dim3(256), 0, stream, p); break;
+        default:
+            if constexpr (DH <= 128) hipLaunchKernelGGL((tree_rows_kernel<DH, 8, 2>), grid, dim3(512), 0, stream, p);
+    }
+    if (p.num_ranges > 1) {
+        const int blocks = row_tile * (DH / 4) / 256;
+        hipLaunchKernelGGL(tree_merge_kernel<DH>, dim3((unsigned)((p.num_ranges - 1) * p.kv_heads), (unsigned)(blocks > 0 ? blocks : 1)),
+                           dim3(256), 0, stream, p, row_tile);
     }
 }
 
@@ -536,20 +677,20 @@ pplhip_retcode launch_tree_attention(const pplhip_tree_attention_args* a, int64_
     p.mask_words = a->tree_mask_words;
     p.num_ranges = (int32_t)ranges;
     p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)a->head_dim));
-    const int nr = tree_row_blocks(a);
-    const uint64_t rows = (uint64_t)p.kv_heads * 2 * (uint64_t)ranges * 16 * nr;
+    const int row_tile = tree_row_tile(a);
+    const uint64_t rows = (uint64_t)p.kv_heads * 2 * (uint64_t)ranges * row_tile;
     p.part_o = (float*)ws;
     p.part_ml = (float2*)(p.part_o + rows * padded_head_dim(a->head_dim));
     p.range_start = (int64_t*)(p.part_ml + rows);
     switch (padded_head_dim(a->head_dim)) {
-        case 32: launch_tree_dh<32>(p, nr, stream); break;
-        case 64: launch_tree_dh<64>(p, nr, stream); break;
-        case 96: launch_tree_dh<96>(p, nr, stream); break;
-        case 128: launch_tree_dh<128>(p, nr, stream); break;
-        case 160: launch_tree_dh<160>(p, nr, stream); break;
-        case 192: launch_tree_dh<192>(p, nr, stream); break;
-        case 224: launch_tree_dh<224>(p, nr, stream); break;
-        default: launch_tree_dh<256>(p, nr, stream); break;
+        case 32: launch_tree_dh<32>(p, row_tile, stream); break;
+        case 64: launch_tree_dh<64>(p, row_tile, stream); break;
+        case 96: launch_tree_dh<96>(p, row_tile, stream); break;
+        case 128: launch_tree_dh<128>(p, row_tile, stream); break;
+        case 160: launch_tree_dh<160>(p, row_tile, stream); break;
+        case 192: launch_tree_dh<192>(p, row_tile, stream); break;
+        case 224: launch_tree_dh<224>(p, row_tile, stream); break;
+        default: launch_tree_dh<256>(p, row_tile, stream); break;
     }
     PPLHIP_CHECK_LAUNCH("tree_attention");
     return PPLHIP_RC_SUCCESS;
