@@ -175,6 +175,8 @@ static pplhip_retcode validate_queries(const Args* a, bool* empty) {
     if (a->total_new_tokens < 0 || a->max_seqlen < 0 || a->max_seqlen > a->total_new_tokens || a->max_kvlen < a->max_seqlen)
         PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "inconsistent sizes: tokens %lld max_seqlen %lld max_kvlen %lld",
                     (long long)a->total_new_tokens, (long long)a->max_seqlen, (long long)a->max_kvlen);
+    if (a->max_kvlen > 0x7fffff00LL || a->total_new_tokens > 0x7fffff00LL / a->num_heads) // (kept in 32 bits)
+        PPLHIP_FAIL(PPLHIP_RC_OUT_OF_RANGE, "too many tokens");
     if (a->batch == 0 || a->total_new_tokens == 0 || a->max_seqlen == 0) {
         *empty = true;
         return PPLHIP_RC_SUCCESS;

@@ -30,11 +30,10 @@ struct CacheView {
 
     // element offset of the K row of key j of sequence b (both wave-uniform; a run of 32 keys from a multiple of 32
     // lies in one page: pages are powers of two of at least 64 tokens)
-    __device__ inline int64_t key_row(int64_t b, int64_t j, int kvh) const {
+    __device__ inline int64_t key_row(int b, int j, int kvh) const {
         const const_tab64_t tab = (const_tab64_t)cachestarts;
         const int64_t t = page_shift == 0 ? tab[b] + j
-                                          : tab[b * cs_stride_b + (j >> page_shift)] +
-                                                (j & ((int64_t(1) << page_shift) - 1));
+                                          : tab[b * cs_stride_b + (j >> page_shift)] + (j & ((1 << page_shift) - 1));
         return addr.row(t, 0, kvh);
     }
 };
@@ -78,6 +77,13 @@ __device__ inline bool piece_is_small(uint32_t scales) { // of the two groups of
     return scale_is_small(s2.x) && scale_is_small(s2.y);
 }
 
+// Offset of a piece in a tile whose last existing row is `last`. Every lane loads something, without a branch: rows past
+// the last repeat it, pieces past head_dim repeat the first (their scales become zeros on the way into LDS). Token
+// strides are below 2^25 elements: 32 of them fit 32 bits.
+__device__ inline uint32_t piece_offset(const CacheView& v, int row, int piece, int last) {
+    return (uint32_t)(row < last ? row : last) * (uint32_t)v.addr.stride_s + (16 * piece < v.head_dim ? 16u * piece : 0u);
+}
+
 template <int DH>
 struct CacheTile {
     static constexpr int PIECES = DH / 16; // 16-byte pieces of a row
@@ -88,35 +94,27 @@ struct CacheTile {
 
     // rows kv0 .. kv0 + 31 from element offset `base`; rows past the sequence's last key (kvlen - 1) repeat it, so that
     // nothing unwritten is ever multiplied
-    __device__ inline void fetch(const CacheView& v, int64_t base, int64_t kv0, int64_t kvlen) {
+    __device__ inline void fetch(const CacheView& v, int64_t base, int kv0, int kvlen) {
         const int lane = threadIdx.x & 63;
-        const int64_t n_left = kvlen - kv0;
-        const int last = n_left < kTileKeys ? (int)n_left - 1 : kTileKeys - 1;
+        const int last = kvlen - kv0 < kTileKeys ? kvlen - kv0 - 1 : kTileKeys - 1;
         const char* cbase = (const char*)v.cache + base;
         const char* sbase = (const char*)v.scale + base / 4; // one fp16 per 8 channels
 #pragma unroll
         for (int n = 0; n < NLD; ++n) {
-            const int c = lane + 64 * n;
-            const int row = c / PIECES, piece = c - row * PIECES;
-            // (token strides are below 2^25 elements: 32 of them fit 32 bits)
-            const uint32_t off = (uint32_t)(row < last ? row : last) * (uint32_t)v.addr.stride_s + 16u * piece;
-            if (16 * piece < v.head_dim) {
-                q[n] = __builtin_nontemporal_load(reinterpret_cast<const uint4_vt*>(cbase + off));
-                s[n] = *reinterpret_cast<const uint32_t*>(sbase + off / 4);
-            } else { // channels past head_dim
-                q[n] = uint4_vt{0, 0, 0, 0};
-                s[n] = 0;
-            }
+            const uint32_t c = lane + 64 * n;
+            const uint32_t off = piece_offset(v, c / PIECES, c % PIECES, last);
+            q[n] = __builtin_nontemporal_load(reinterpret_cast<const uint4_vt*>(cbase + off));
+            s[n] = *reinterpret_cast<const uint32_t*>(sbase + off / 4);
         }
     }
 
-    __device__ inline void stash(half_t* tile) const {
+    __device__ inline void stash(half_t* tile, int head_dim) const {
         const int lane = threadIdx.x & 63;
 #pragma unroll
         for (int n = 0; n < NLD; ++n) {
-            const int c = lane + 64 * n;
-            const int row = c / PIECES, piece = c - row * PIECES;
-            const half2_t s2 = as_half2(s[n]);
+            const uint32_t c = lane + 64 * n;
+            const int row = c / PIECES, piece = c % PIECES;
+            const half2_t s2 = as_half2(16 * piece < head_dim ? s[n] : 0u);
             half8_t* dst = reinterpret_cast<half8_t*>(tile + row * LDR + 16 * piece);
             dst[0] = dequant8(q[n].x, q[n].y, s2.x);
             dst[1] = dequant8(q[n].z, q[n].w, s2.y);
@@ -134,11 +132,11 @@ struct CacheTile {
         return rows;
     }
     // as stash, with zeros for the pieces that may hold such values
-    __device__ inline void stash_finite(half_t* tile) const {
+    __device__ inline void stash_finite(half_t* tile, int head_dim) const {
         CacheTile<DH> t = *this;
 #pragma unroll
         for (int n = 0; n < NLD; ++n) t.s[n] = piece_is_small(s[n]) ? s[n] : 0u;
-        t.stash(tile);
+        t.stash(tile, head_dim);
     }
 };
 
@@ -152,37 +150,35 @@ struct SharedTile {
     uint4_vt q[NLD];
     uint32_t s[NLD];
 
+    // Piece n of this thread: K or V (the same for the whole wave: a tile's K pieces are a multiple of 64), row, piece of it
+    __device__ static inline void place(int n, int* kv, int* row, int* piece) {
+        const int first = 64 * (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) + W * n); // the wave's first piece
+        *kv = first >= kTileKeys * PIECES;
+        const uint32_t c = (threadIdx.x & 63) + first - (*kv ? kTileKeys * PIECES : 0);
+        *row = c / PIECES;
+        *piece = c % PIECES;
+    }
     // base: element offset of the tile's first K row
-    __device__ inline void fetch(const CacheView& v, int64_t base, int64_t kv0, int64_t kvlen) {
-        const int64_t n_left = kvlen - kv0;
-        const int last = n_left < kTileKeys ? (int)n_left - 1 : kTileKeys - 1;
+    __device__ inline void fetch(const CacheView& v, int64_t base, int kv0, int kvlen) {
+        const int last = kvlen - kv0 < kTileKeys ? kvlen - kv0 - 1 : kTileKeys - 1;
 #pragma unroll
         for (int n = 0; n < NLD; ++n) {
-            const int c = threadIdx.x + 64 * W * n;
-            const int kv = c >= kTileKeys * PIECES;
-            const int c2 = c - kv * kTileKeys * PIECES;
-            const int row = c2 / PIECES, piece = c2 - row * PIECES;
-            if (c < ALL && 16 * piece < v.head_dim) {
-                const int64_t off = base + (kv ? v.addr.stride_kv : 0) +
-                                    (int64_t)(row < last ? row : last) * v.addr.stride_s + 16 * piece;
-                q[n] = __builtin_nontemporal_load(reinterpret_cast<const uint4_vt*>(v.cache + off));
-                s[n] = *reinterpret_cast<const uint32_t*>((const char*)v.scale + off / 4);
-            } else {
-                q[n] = uint4_vt{0, 0, 0, 0};
-                s[n] = 0;
-            }
+            int kv, row, piece;
+            place(n, &kv, &row, &piece);
+            const int64_t first = base + (kv ? v.addr.stride_kv : 0);
+            const uint32_t off = piece_offset(v, row, piece, last);
+            q[n] = __builtin_nontemporal_load(reinterpret_cast<const uint4_vt*>((const char*)v.cache + first + off));
+            s[n] = *reinterpret_cast<const uint32_t*>((const char*)v.scale + first / 4 + off / 4);
         }
     }
     // odd: where to note the V rows with pieces that may not be finite (those become zeros); null: not looked at
-    __device__ inline void stash(half_t* k_tile, half_t* v_tile, uint32_t* odd) const {
+    __device__ inline void stash(half_t* k_tile, half_t* v_tile, int head_dim, uint32_t* odd) const {
 #pragma unroll
         for (int n = 0; n < NLD; ++n) {
-            const int c = threadIdx.x + 64 * W * n;
-            if (ALL % (64 * W) != 0 && c >= ALL) break;
-            const int kv = c >= kTileKeys * PIECES;
-            const int c2 = c - kv * kTileKeys * PIECES;
-            const int row = c2 / PIECES, piece = c2 - row * PIECES;
-            uint32_t sc = s[n];
+            int kv, row, piece;
+            place(n, &kv, &row, &piece);
+            if (row >= kTileKeys) break;
+            uint32_t sc = 16 * piece < head_dim ? s[n] : 0u;
             if (odd && kv && !piece_is_small(sc)) {
                 sc = 0;
                 atomicOr(odd, 1u << row);

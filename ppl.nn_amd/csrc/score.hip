@@ -63,13 +63,13 @@ __global__ __launch_bounds__(256, 2) void kv_score_kernel(const ScoreParams p) {
         CacheTile<DH> raw[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int64_t kv0 = key0 + h * kTileKeys < kvlen ? key0 + h * kTileKeys : key0;
-            raw[h].fetch(p.view, p.view.key_row(b, kv0, kvh), kv0, kvlen);
+            const int kv0 = (int)(key0 + h * kTileKeys < kvlen ? key0 + h * kTileKeys : key0);
+            raw[h].fetch(p.view, p.view.key_row(b, kv0, kvh), kv0, (int)kvlen);
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             wave_lds_order();
-            raw[h].stash(tile);
+            raw[h].stash(tile, hd);
             wave_lds_order();
 #pragma unroll
             for (int i = 0; i < 2; ++i)

@@ -74,7 +74,8 @@ __device__ inline TreeSpan tree_span(const TreeParams& p, int b, int rows_per_ti
 
 struct RangeStart {
     int32_t b;
-    int64_t row_tile, key_tile, length; // length: positions of the axis in this range
+    int32_t row_tile, key_tile;
+    int64_t length; // positions of the axis in this range
 };
 
 // Where range `r` starts. Every wave works it out alone: 64 sequences' costs a step, summed and scanned across the lanes.
@@ -105,10 +106,10 @@ __device__ inline RangeStart find_range(const TreeParams& p, int r, int rows_per
             const int who = __ffsll((unsigned long long)here) - 1;
             const int64_t start = before + __shfl(incl - sp.cost(), who);
             const int64_t per_tile = __shfl(sp.key_tiles, who) + kPieceCost;
-            s.b = __builtin_amdgcn_readfirstlane(b0 + who);
-            s.row_tile = uniform64((pos - start) / per_tile);
-            s.key_tile = uniform64((pos - start) % per_tile);
-            s.length = uniform64(len < total - pos ? len : total - pos);
+            s.b = b0 + who;
+            s.row_tile = (int)((pos - start) / per_tile);
+            s.key_tile = (int)((pos - start) % per_tile);
+            s.length = len < total - pos ? len : total - pos;
             return s;
         }
         before += __shfl(incl, 63);
@@ -116,26 +117,20 @@ __device__ inline RangeStart find_range(const TreeParams& p, int r, int rows_per
     return s;
 }
 
-// Bit i: the row sees key kv0 + i (i < 32). `start`: cached tokens in front of the new ones.
-__device__ inline uint32_t visible_keys(const uint64_t* row_mask, int words, int64_t token, int64_t kv0, int64_t start,
-                                        int64_t kvlen) {
-    if (kv0 + kTileKeys <= start) return ~0u;
-    const int64_t i0 = kv0 - start; // new-token index of the tile's first key (negative: history in front)
+// Bit i: the row sees key kv0 + i (i < 32). `start`: cached tokens in front of the new ones; kv0 + 32 > start.
+__device__ inline uint32_t visible_keys(const uint64_t* row_mask, int words, int token, int kv0, int start, int kvlen) {
+    const int i0 = kv0 - start; // new-token index of the tile's first key (negative: history in front)
     if (!row_mask) {
-        const int64_t n = token - i0 + 1;
+        const int n = token - i0 + 1;
         return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1;
     }
-    const int64_t first = i0 < 0 ? 0 : i0;
-    const int64_t w = first >> 6;
-    const int sh = (int)(first & 63);
+    const int first = i0 < 0 ? 0 : i0;
+    const int w = first >> 6, sh = first & 63;
     uint64_t bits = w < words ? row_mask[w] >> sh : 0;
     if (sh > 32 && w + 1 < words) bits |= row_mask[w + 1] << (64 - sh);
     uint32_t see = (uint32_t)bits;
-    if (i0 < 0) {
-        const int hist = (int)-i0; // 1 .. 31
-        see = (see << hist) | ((1u << hist) - 1);
-    }
-    const int64_t n = kvlen - kv0;
+    if (i0 < 0) see = (see << -i0) | ((1u << -i0) - 1); // (-i0 is 1 .. 31)
+    const int n = kvlen - kv0;
     return n >= 32 ? see : see & ((1u << n) - 1);
 }
 
@@ -143,23 +138,20 @@ __device__ inline uint32_t visible_keys(const uint64_t* row_mask, int words, int
 // channels 16 i + 4 g .. + 3 and of the sum its own keys' share.
 template <int DH, int N>
 struct RowState {
-    int64_t tok[N];
-    int head[N];
-    bool valid[N];
+    int tok[N]; // token of the sequence; -1 for rows past the last one
     half8_t qf[N][DH / 32];
     float m[N], shift[N], l[N]; // m in units of the raw products; shift = kProbShift - m * scale_log2
     float4_t o[N][DH / 16];
 
-    __device__ inline void start(const TreeParams& p, int64_t s0, int64_t rows, const int64_t (&first_row)[N], int kvh) {
+    __device__ inline void start(const TreeParams& p, int64_t s0, int rows, const int (&first_row)[N], int kvh) {
         const int lane = threadIdx.x & 63, g = lane >> 4;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int64_t row = first_row[n] + (lane & 15);
-            valid[n] = row < rows;
-            const int64_t rr = valid[n] ? row : rows - 1;
-            tok[n] = (uint64_t)rr >> 32 ? rr / p.rep : (int64_t)((uint32_t)rr / (uint32_t)p.rep);
-            head[n] = kvh * p.rep + (int)(rr - tok[n] * p.rep);
-            const half_t* qp = p.q + ((s0 + tok[n]) * p.num_heads + head[n]) * p.view.head_dim + 8 * g;
+            const int row = first_row[n] + (lane & 15);
+            const int rr = row < rows ? row : rows - 1;
+            const int t = rr / p.rep;
+            tok[n] = row < rows ? t : -1;
+            const half_t* qp = p.q + ((s0 + t) * p.num_heads + kvh * p.rep + (rr - t * p.rep)) * p.view.head_dim + 8 * g;
 #pragma unroll
             for (int kc = 0; kc < DH / 32; ++kc) {
                 if (32 * kc + 8 * g < p.view.head_dim) {
@@ -175,6 +167,15 @@ struct RowState {
 #pragma unroll
             for (int i = 0; i < DH / 16; ++i) o[n][i] = float4_t{0.f, 0.f, 0.f, 0.f};
         }
+    }
+
+    // Waits for the queries here, while younger loads stay in flight: what is known about loads in flight is merged at a
+    // loop's head, and a load that is first used inside the loop is waited for there with everything behind it.
+    __device__ inline void queries_here() {
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int kc = 0; kc < DH / 32; ++kc) asm volatile("" : "+v"(qf[n][kc]));
     }
 
     // scores of the rows against the 32 keys in `tile`: s[n][tb][e] belongs to key 16 * tb + 4 * g + e
@@ -200,12 +201,12 @@ struct RowState {
     }
 
     // keys a row does not see get score -inf; see[n]: bit i = key kv0 + i
-    __device__ inline void hide(const TreeParams& p, int64_t s0, int64_t kv0, int64_t start, int64_t kvlen,
+    __device__ inline void hide(const TreeParams& p, int64_t s0, int kv0, int start, int kvlen,
                                 float (&s)[N][2][4], uint32_t (&see)[N]) const {
         const int g = (threadIdx.x & 63) >> 4;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            see[n] = valid[n] ? visible_keys(p.mask ? p.mask + (s0 + tok[n]) * p.mask_words : nullptr, p.mask_words, tok[n],
+            see[n] = tok[n] >= 0 ? visible_keys(p.mask ? p.mask + (s0 + tok[n]) * p.mask_words : nullptr, p.mask_words, tok[n],
                                              kv0, start, kvlen)
                               : 0u;
             const uint32_t mine = see[n] >> (4 * g);
@@ -216,8 +217,8 @@ struct RowState {
         }
     }
 
-    // scores -> weights (left in s, and as fp16 in pp), running sums
-    __device__ inline void weights(float scale_log2, float (&s)[N][2][4], half8_t (&pp)[N]) {
+    // scores -> weights (fp16, the operand of the second product), running sums
+    __device__ inline void weights(float scale_log2, const float (&s)[N][2][4], half8_t (&pp)[N]) {
         float top[N];
         bool moves = false;
 #pragma unroll
@@ -249,7 +250,6 @@ struct RowState {
                 for (int e = 0; e < 4; ++e) {
                     const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][tb][e], scale_log2, shift[n]));
                     sum += w;
-                    s[n][tb][e] = w;
                     pp[n][4 * tb + e] = (half_t)w;
                 }
             l[n] += sum;
@@ -276,31 +276,32 @@ struct RowState {
     }
 
     // Value pieces that may not be finite are zeros in the tile (a key can be hidden from a row: its weight there is 0,
-    // and 0 times a NaN or an infinity is NaN): they are added here, to the rows that see their key. rows: which rows of
-    // the tile have such pieces; base: element offset of its first V row.
-    __device__ inline void odd_values(const TreeParams& p, int64_t base, int64_t kv0, int64_t kvlen, uint32_t rows,
-                                      const float (&s)[N][2][4], const uint32_t (&see)[N]) {
+    // and 0 times a NaN or an infinity is NaN). Here they are multiplied key by key, and the result is taken over by the
+    // rows that see the key only. rows: which rows of the tile have such pieces; base: offset of its first V row.
+    __device__ inline void odd_values(const TreeParams& p, int64_t base, int kv0, int kvlen, uint32_t rows,
+                                      const half8_t (&pp)[N], const uint32_t (&see)[N]) {
         const int lane = threadIdx.x & 63, g = lane >> 4;
+#pragma unroll 1
         for (; rows; rows &= rows - 1) {
             const int row = __builtin_ctz(rows);
             if (kv0 + row >= kvlen) break;
             const int8_t* vq = p.view.cache + base + row * p.view.addr.stride_s;
             const half_t* vs = p.view.scale + (base + row * p.view.addr.stride_s) / kQuantGroup;
+            const int slot = (row & 3) + 4 * (row >> 4); // where lane group (row >> 2) & 3 holds the key
 #pragma unroll
-            for (int n = 0; n < N; ++n) {
-                float w = 0.f;
+            for (int i = 0; i < DH / 16; ++i) {
+                __builtin_amdgcn_sched_barrier(0);
+                if (16 * i >= p.view.head_dim || (scale_is_small(vs[2 * i]) && scale_is_small(vs[2 * i + 1]))) continue;
+                const int d = 16 * i + (lane & 15);
+                const half_t v = (half_t)((float)vq[d] * (float)vs[d >> 3]);
+                half8_t a;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) w = (row & 3) + 4 * (row >> 4) == k ? s[n][k >> 2][k & 3] : w;
-                w = (float)(half_t)__shfl(w, 16 * ((row >> 2) & 3) + (lane & 15));
-                if (!((see[n] >> row) & 1)) continue;
+                for (int e = 0; e < 8; ++e) a[e] = g == ((row >> 2) & 3) && e == slot ? v : (half_t)0.f;
 #pragma unroll
-                for (int i = 0; i < DH / 16; ++i) {
-                    if (16 * i >= p.view.head_dim || (scale_is_small(vs[2 * i]) && scale_is_small(vs[2 * i + 1]))) continue;
+                for (int n = 0; n < N; ++n) {
+                    const float4_t with = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pp[n], o[n][i], 0, 0, 0);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int d = 16 * i + 4 * g + e;
-                        o[n][i][e] += w * (float)(half_t)((float)vq[d] * (float)vs[d >> 3]);
-                    }
+                    for (int e = 0; e < 4; ++e) o[n][i][e] = (see[n] >> row) & 1 ? with[e] : o[n][i][e];
                 }
             }
         }
@@ -308,9 +309,9 @@ struct RowState {
 };
 
 // Writes 4 channels of a finished row, and its log-sum with channel 0. l == 0: the row saw nothing (a NaN stays NaN).
-__device__ inline void finish_row(const TreeParams& p, int64_t s0, int64_t row, int kvh, int d, float4_t a, float m_log2,
+__device__ inline void finish_row(const TreeParams& p, int64_t s0, int row, int kvh, int d, float4_t a, float m_log2,
                                   float l) {
-    const int64_t t = row / p.rep;
+    const int t = row / p.rep;
     const int64_t at = (s0 + t) * p.num_heads + kvh * p.rep + (row - t * p.rep);
     const float inv = l != 0.f ? 1.0f / l : 0.f;
     const half4_t r = {(half_t)(a[0] * inv), (half_t)(a[1] * inv), (half_t)(a[2] * inv), (half_t)(a[3] * inv)};
@@ -321,8 +322,9 @@ __device__ inline void finish_row(const TreeParams& p, int64_t s0, int64_t row, 
 // One (sequence, row tile) piece of a range, as far as both kernels agree on it.
 struct TreePiece {
     int32_t b;
-    int64_t s0, start, kvlen, rows, row0; // row0: first row of the tile
-    int64_t key_tile, stop_tile; // key tiles to look at (causal rows see nothing past their own token)
+    int64_t s0;
+    int32_t start, kvlen, rows, row0; // row0: first row of the tile
+    int32_t key_tile, stop_tile; // key tiles to look at (causal rows see nothing past their own token)
     bool whole; // all the row tile's keys are in this piece
     int64_t slot; // else: where its partial goes
 };
@@ -332,25 +334,26 @@ template <int ROWS, class F>
 __device__ inline void walk_range(const TreeParams& p, int range, int kvh, F&& piece) {
     const const_tab64_t seqstarts = (const_tab64_t)p.seqstarts, kvstarts = (const_tab64_t)p.kvstarts;
     const RangeStart rs = find_range(p, range, ROWS);
-    int64_t left = rs.length;
-    int b = rs.b;
-    int64_t row_tile = rs.row_tile, key_tile = rs.key_tile;
-    int64_t first_b = -1, first_row_tile = 0, first_key_tile = 0;
+    // (every lane found the same; said here, so that what follows from it is scalar)
+    int64_t left = uniform64(rs.length);
+    int b = __builtin_amdgcn_readfirstlane(rs.b), row_tile = __builtin_amdgcn_readfirstlane(rs.row_tile),
+        key_tile = __builtin_amdgcn_readfirstlane(rs.key_tile);
+    int first_b = -1, first_row_tile = 0, first_key_tile = 0;
     while (left > 0 && b < p.batch) {
         TreePiece t;
         t.b = b;
         t.s0 = seqstarts[b];
-        const int64_t L = seqstarts[b + 1] - t.s0;
-        t.kvlen = kvstarts[b + 1] - kvstarts[b];
+        const int L = (int)(seqstarts[b + 1] - t.s0);
+        t.kvlen = (int)(kvstarts[b + 1] - kvstarts[b]);
         t.rows = L * p.rep;
-        const int64_t row_tiles = L <= 0 ? 0 : (t.rows + ROWS - 1) / ROWS;
-        const int64_t key_tiles = (t.kvlen + kTileKeys - 1) / kTileKeys;
+        const int row_tiles = L <= 0 ? 0 : (t.rows + ROWS - 1) / ROWS;
+        const int key_tiles = (t.kvlen + kTileKeys - 1) / kTileKeys;
         if (row_tile >= row_tiles) {
             ++b;
             row_tile = key_tile = 0;
             continue;
         }
-        const int64_t end_tile = key_tile + left < key_tiles ? key_tile + left : key_tiles;
+        const int end_tile = key_tile + left < key_tiles ? key_tile + (int)left : key_tiles;
         if (key_tile < end_tile) {
             if (first_b < 0) {
                 first_b = b;
@@ -362,8 +365,8 @@ __device__ inline void walk_range(const TreeParams& p, int range, int kvh, F&& p
             t.key_tile = key_tile;
             t.stop_tile = end_tile;
             if (!p.mask) {
-                const int64_t last_row = t.row0 + ROWS < t.rows ? t.row0 + ROWS - 1 : t.rows - 1;
-                const int64_t last = (t.start + last_row / p.rep + kTileKeys) / kTileKeys;
+                const int last_row = t.row0 + ROWS < t.rows ? t.row0 + ROWS - 1 : t.rows - 1;
+                const int last = (t.start + last_row / p.rep + kTileKeys) / kTileKeys;
                 t.stop_tile = last < end_tile ? last : end_tile;
             }
             t.whole = key_tile == 0 && end_tile == key_tiles;
@@ -405,31 +408,28 @@ __global__ __launch_bounds__(256, tree_waves_per_simd(DH, NR)) void tree_keys_ke
 
     walk_range<ROWS>(p, range, kvh, [&](const TreePiece& t) {
         RowState<DH, NR> st;
-        int64_t first_row[NR];
+        int first_row[NR];
 #pragma unroll
         for (int n = 0; n < NR; ++n) first_row[n] = t.row0 + 16 * n;
         st.start(p, t.s0, t.rows, first_row, kvh);
 
         CacheTile<DH> rk, rv; // the next tile's K and V rows, on their way
-        int64_t kt = t.key_tile + wave;
-        int64_t base = 0, base_now = 0;
-        if (kt < t.stop_tile) {
-            base = p.view.key_row(t.b, kt * kTileKeys, kvh);
-            rk.fetch(p.view, base, kt * kTileKeys, t.kvlen);
-            rv.fetch(p.view, base + p.view.addr.stride_kv, kt * kTileKeys, t.kvlen);
-        }
+        int kt = t.key_tile + wave;
+        const int first_key = (kt < t.stop_tile ? kt : t.key_tile) * kTileKeys; // (a wave without a tile: any)
+        int64_t base = p.view.key_row(t.b, first_key, kvh), base_now = base;
+        rk.fetch(p.view, base, first_key, t.kvlen);
+        rv.fetch(p.view, base + p.view.addr.stride_kv, first_key, t.kvlen);
+        st.queries_here();
         for (; kt < t.stop_tile; kt += kTreeWaves) {
-            const int64_t kv0 = kt * kTileKeys, kv_next = kv0 + kTreeWaves * kTileKeys;
-            const bool more = kt + kTreeWaves < t.stop_tile;
+            const int kv0 = kt * kTileKeys;
+            const int kv_next = kt + kTreeWaves < t.stop_tile ? kv0 + kTreeWaves * kTileKeys : kv0; // (the last: again)
             const bool history = kv0 + kTileKeys <= t.start; // every row sees every key
             base_now = base;
             wave_lds_order();
-            rk.stash(tile);
+            rk.stash(tile, p.view.head_dim);
             wave_lds_order();
-            if (more) {
-                base = p.view.key_row(t.b, kv_next, kvh);
-                rk.fetch(p.view, base, kv_next, t.kvlen);
-            }
+            base = p.view.key_row(t.b, kv_next, kvh);
+            rk.fetch(p.view, base, kv_next, t.kvlen);
             float s[NR][2][4];
             uint32_t see[NR];
             half8_t pp[NR];
@@ -439,13 +439,13 @@ __global__ __launch_bounds__(256, tree_waves_per_simd(DH, NR)) void tree_keys_ke
             const uint32_t odd = history ? 0u : rv.odd_rows();
             wave_lds_order();
             if (odd)
-                rv.stash_finite(tile);
+                rv.stash_finite(tile, p.view.head_dim);
             else
-                rv.stash(tile);
+                rv.stash(tile, p.view.head_dim);
             wave_lds_order();
-            if (more) rv.fetch(p.view, base + p.view.addr.stride_kv, kv_next, t.kvlen);
+            rv.fetch(p.view, base + p.view.addr.stride_kv, kv_next, t.kvlen);
             st.values(tile, pp);
-            if (odd) st.odd_values(p, base_now + p.view.addr.stride_kv, kv0, t.kvlen, odd, s, see);
+            if (odd) st.odd_values(p, base_now + p.view.addr.stride_kv, kv0, t.kvlen, odd, pp, see);
         }
 
         // ---- the four waves' shares of the piece, joined 16 rows at a time
@@ -478,7 +478,7 @@ __global__ __launch_bounds__(256, tree_waves_per_simd(DH, NR)) void tree_keys_ke
                     l += ml.y * __builtin_amdgcn_exp2f(ml.x - (mm == -INFINITY ? 0.f : mm));
                     a += *reinterpret_cast<const float4_t*>(olds + (w * 16 + r) * LDO + d);
                 }
-                const int64_t row = t.row0 + 16 * n + r;
+                const int row = t.row0 + 16 * n + r;
                 if (t.whole) {
                     if (row < t.rows && d < p.view.head_dim) finish_row(p, t.s0, row, kvh, d, a, mm, l);
                 } else {
@@ -510,34 +510,40 @@ __global__ __launch_bounds__(W * 64, tree_waves_per_simd(DH, NB)) void tree_rows
 
     walk_range<ROWS>(p, range, kvh, [&](const TreePiece& t) {
         RowState<DH, NB> st;
-        int64_t first_row[NB];
+        int first_row[NB];
 #pragma unroll
         for (int n = 0; n < NB; ++n) first_row[n] = t.row0 + 16 * (wave + W * n);
         st.start(p, t.s0, t.rows, first_row, kvh);
         const bool busy = first_row[0] < t.rows; // (a wave without rows only helps to bring the tiles)
-        const int n_tiles = (int)(t.stop_tile - t.key_tile);
+        const int n_tiles = t.stop_tile - t.key_tile;
 
         SharedTile<DH, W> raw[2]; // tiles i + 1 and i + 2, on their way
-        auto fetch = [&](SharedTile<DH, W>& r, int i) {
-            const int64_t kv0 = (t.key_tile + i) * kTileKeys;
+        auto fetch = [&](SharedTile<DH, W>& r, int i) { // (past the last tile: that one again, so that every path has
+                                                        // the same loads in flight and none is waited for too early)
+            const int kv0 = (t.key_tile + (i < n_tiles ? i : n_tiles - 1)) * kTileKeys;
             r.fetch(p.view, p.view.key_row(t.b, kv0, kvh), kv0, t.kvlen);
         };
         auto stash = [&](const SharedTile<DH, W>& r, int i) {
             const bool history = (t.key_tile + i + 1) * kTileKeys <= t.start;
-            r.stash(lds[i & 1][0], lds[i & 1][1], history ? nullptr : &odd_lds[i % 3]);
+            r.stash(lds[i & 1][0], lds[i & 1][1], p.view.head_dim, history ? nullptr : &odd_lds[i % 3]);
         };
         __syncthreads(); // (the piece before has read its last tile)
         if (threadIdx.x < 3) odd_lds[threadIdx.x] = 0;
-        if (n_tiles > 0) fetch(raw[0], 0);
-        if (n_tiles > 1) fetch(raw[1], 1);
+        if (n_tiles > 0) {
+            fetch(raw[0], 0);
+            fetch(raw[1], 1);
+        }
+        st.queries_here();
         __syncthreads();
-        if (n_tiles > 0) stash(raw[0], 0);
-        if (n_tiles > 2) fetch(raw[0], 2);
+        if (n_tiles > 0) {
+            stash(raw[0], 0);
+            fetch(raw[0], 2);
+        }
         __syncthreads();
         auto step = [&](SharedTile<DH, W>& next, int i) { // next: tile i + 1, then tile i + 3
             if (threadIdx.x == 0) odd_lds[(i + 2) % 3] = 0;
             if (busy) {
-                const int64_t kv0 = (t.key_tile + i) * kTileKeys;
+                const int kv0 = (t.key_tile + i) * kTileKeys;
                 const bool history = kv0 + kTileKeys <= t.start;
                 float s[NB][2][4];
                 uint32_t see[NB];
@@ -548,15 +554,19 @@ __global__ __launch_bounds__(W * 64, tree_waves_per_simd(DH, NB)) void tree_rows
                 st.values(lds[i & 1][1], pp);
                 const uint32_t odd = history ? 0u : __builtin_amdgcn_readfirstlane(odd_lds[i % 3]);
                 if (odd)
-                    st.odd_values(p, p.view.key_row(t.b, kv0, kvh) + p.view.addr.stride_kv, kv0, t.kvlen, odd, s, see);
+                    st.odd_values(p, p.view.key_row(t.b, kv0, kvh) + p.view.addr.stride_kv, kv0, t.kvlen, odd, pp, see);
             }
-            if (i + 1 < n_tiles) stash(next, i + 1);
-            if (i + 3 < n_tiles) fetch(next, i + 3);
+            stash(next, i + 1); // (past the last tile: into the buffer nobody reads any more)
+            fetch(next, i + 3);
             __syncthreads();
         };
-        for (int i = 0; i < n_tiles; i += 2) {
-            step(raw[1], i);
-            if (i + 1 < n_tiles) step(raw[0], i + 1);
+        if (n_tiles > 0) {
+            for (int i = 0;;) { // (left from the middle, so that at its head raw[1] is always the older of the two)
+                step(raw[1], i);
+                if (++i >= n_tiles) break;
+                step(raw[0], i);
+                if (++i >= n_tiles) break;
+            }
         }
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
@@ -565,9 +575,9 @@ __global__ __launch_bounds__(W * 64, tree_waves_per_simd(DH, NB)) void tree_rows
             if (t.whole) {
 #pragma unroll
                 for (int i = 0; i < DH / 16; ++i)
-                    if (st.valid[n] && 16 * i < p.view.head_dim)
+                    if (st.tok[n] >= 0 && 16 * i < p.view.head_dim)
                         finish_row(p, t.s0, t.row0 + r, kvh, 16 * i + 4 * g, st.o[n][i], st.m[n] * p.scale_log2, l);
-            } else if (st.valid[n]) {
+            } else if (st.tok[n] >= 0) {
                 const int64_t at = t.slot * ROWS + r;
 #pragma unroll
                 for (int i = 0; i < DH / 16; ++i)
@@ -596,7 +606,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeParams p, con
     const int64_t base = (int64_t)kvh * 2 * p.num_ranges;
     for (int x = blockIdx.y * 256 + threadIdx.x; x < ROWS * (DH / 4); x += 256 * gridDim.y) {
         const int r = x / (DH / 4), d = (x - r * (DH / 4)) * 4;
-        const int64_t row = row_tile * ROWS + r;
+        const int row = (int)row_tile * ROWS + r;
         if (row >= rows || d >= p.view.head_dim) continue;
         float m = -INFINITY, l = 0.f;
         float4_t a = {0.f, 0.f, 0.f, 0.f};
