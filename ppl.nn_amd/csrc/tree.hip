@@ -151,16 +151,10 @@ struct RowState {
             const int rr = row < rows ? row : rows - 1;
             const int t = rr / p.rep;
             tok[n] = row < rows ? t : -1;
-            const half_t* qp = p.q + ((s0 + t) * p.num_heads + kvh * p.rep + (rr - t * p.rep)) * p.view.head_dim + 8 * g;
+            const half_t* qp = p.q + ((s0 + t) * p.num_heads + kvh * p.rep + (rr - t * p.rep)) * p.view.head_dim;
 #pragma unroll
-            for (int kc = 0; kc < DH / 32; ++kc) {
-                if (32 * kc + 8 * g < p.view.head_dim) {
-                    qf[n][kc] = *reinterpret_cast<const half8_t*>(qp + 32 * kc);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) qf[n][kc][e] = (half_t)0.f;
-                }
-            }
+            for (int kc = 0; kc < DH / 32; ++kc) // (groups past head_dim: the first one, zeroed in queries_here)
+                qf[n][kc] = *reinterpret_cast<const half8_t*>(qp + (32 * kc + 8 * g < p.view.head_dim ? 32 * kc + 8 * g : 0));
             m[n] = -INFINITY;
             shift[n] = kProbShift;
             l[n] = 0.f;
@@ -171,11 +165,16 @@ struct RowState {
 
     // Waits for the queries here, while younger loads stay in flight: what is known about loads in flight is merged at a
     // loop's head, and a load that is first used inside the loop is waited for there with everything behind it.
-    __device__ inline void queries_here() {
+    __device__ inline void queries_here(int head_dim) {
+        const int g = (threadIdx.x & 63) >> 4;
 #pragma unroll
-        for (int n = 0; n < N; ++n)
+        for (int n = 0; n < N; ++n) {
 #pragma unroll
-            for (int kc = 0; kc < DH / 32; ++kc) asm volatile("" : "+v"(qf[n][kc]));
+            for (int kc = 0; kc < DH / 32; ++kc) {
+                asm volatile("" : "+v"(qf[n][kc]));
+                if (head_dim < DH && 32 * kc + 8 * g >= head_dim) qf[n][kc] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
+            }
+        }
     }
 
     // scores of the rows against the 32 keys in `tile`: s[n][tb][e] belongs to key 16 * tb + 4 * g + e
@@ -384,9 +383,10 @@ __device__ inline void walk_range(const TreeParams& p, int range, int kvh, F&& p
     }
 }
 
-// What the register allocator is to leave room for: above head_dim 128 two row blocks need more than half a SIMD's registers.
+// Waves per SIMD that the register allocator is to leave room for: what a wave's N row blocks, the tiles on their way and
+// the operands of one product take without spilling.
 constexpr int tree_waves_per_simd(int dh, int row_blocks) {
-    return dh > 128 && row_blocks > 1 ? 1 : 2;
+    return row_blocks == 1 ? (dh <= 128 ? 3 : 2) : (dh <= 128 ? 2 : 1);
 }
 
 // NR: blocks of 16 rows every wave carries; the row tile has 16 * NR rows.
@@ -419,7 +419,7 @@ __global__ __launch_bounds__(256, tree_waves_per_simd(DH, NR)) void tree_keys_ke
         int64_t base = p.view.key_row(t.b, first_key, kvh), base_now = base;
         rk.fetch(p.view, base, first_key, t.kvlen);
         rv.fetch(p.view, base + p.view.addr.stride_kv, first_key, t.kvlen);
-        st.queries_here();
+        st.queries_here(p.view.head_dim);
         for (; kt < t.stop_tile; kt += kTreeWaves) {
             const int kv0 = kt * kTileKeys;
             const int kv_next = kt + kTreeWaves < t.stop_tile ? kv0 + kTreeWaves * kTileKeys : kv0; // (the last: again)
@@ -533,7 +533,7 @@ __global__ __launch_bounds__(W * 64, tree_waves_per_simd(DH, NB)) void tree_rows
             fetch(raw[0], 0);
             fetch(raw[1], 1);
         }
-        st.queries_here();
+        st.queries_here(p.view.head_dim);
         __syncthreads();
         if (n_tiles > 0) {
             stash(raw[0], 0);
@@ -634,13 +634,15 @@ int tree_row_tile(const pplhip_tree_attention_args* a) {
     return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 || a->head_dim > 128 ? 128 : 256;
 }
 
-// As many ranges as workgroups are resident (two per CU), shared out among the kv heads; never more than ranges of the
-// least length in the longest possible axis.
+// As many ranges as workgroups are resident, shared out among the kv heads; never more than ranges of the least length in
+// the longest possible axis.
 int64_t tree_num_ranges(const pplhip_tree_attention_args* a, int cu_count) {
     const int64_t rep = a->num_heads / a->num_kv_heads;
     const int64_t row_tiles = (a->max_seqlen * rep + tree_row_tile(a) - 1) / tree_row_tile(a);
     const int64_t key_tiles = (a->max_kvlen + kTileKeys - 1) / kTileKeys;
-    int64_t ranges = (int64_t)cu_count * 2 / a->num_kv_heads;
+    const int row_blocks = tree_row_tile(a) == 16 || tree_row_tile(a) == 64 ? 1 : 2;
+    const int per_cu = tree_waves_per_simd(padded_head_dim(a->head_dim), row_blocks) / (tree_row_tile(a) == 256 ? 2 : 1);
+    int64_t ranges = (int64_t)cu_count * per_cu / a->num_kv_heads;
     const double most = (double)a->batch * (double)row_tiles * (double)(key_tiles + kPieceCost) / kMinRangeTiles;
     if ((double)ranges > most) ranges = (int64_t)most + 1;
     return ranges < 1 ? 1 : ranges;
