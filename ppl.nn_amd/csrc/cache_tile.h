@@ -3,9 +3,13 @@
 //
 // A lane loads 16-byte pieces (two quantisation groups), consecutive lanes consecutive pieces of a row, so that one load
 // instruction covers whole 128-byte lines, and with them the two groups' scales (4 bytes). Dequantisation happens in that
-// orientation, where a group's scale is one value: fp16(float(q) * float(scale)), as everywhere. Rows have DH channels in
-// LDS (head_dim rounded up to a multiple of 32, zeros past head_dim) and are padded by 8 halves: 16-byte reads of 16
-// rows at one column, and the writes, then touch every bank once.
+// orientation, where a group's scale is one value: fp16(float(q) * float(scale)), as everywhere.
+//
+// In LDS a row has DH channels (head_dim rounded up to a multiple of 32, zeros past head_dim) in units of one group (16
+// bytes): first the pieces' even groups, then their odd ones, so that the lanes of a row write 16 consecutive units at a
+// time. Which channel a position holds (channel_at) only matters where queries are loaded and outputs stored. K rows are
+// padded by one unit, V rows by two: the 16-byte reads of 16 K rows at one position, and the transposing 8-byte reads of
+// four V rows, then touch every bank once.
 #ifndef PPLHIP_CSRC_CACHE_TILE_H_
 #define PPLHIP_CSRC_CACHE_TILE_H_
 
@@ -17,6 +21,19 @@ typedef uint32_t uint4_vt __attribute__((ext_vector_type(4)));
 typedef const int64_t __attribute__((address_space(4)))* const_tab64_t; // wave-uniform reads are scalar loads
 
 constexpr int kTileKeys = 32;
+
+template <int DH>
+constexpr int kKeyRow = DH + 8; // halves per K row in LDS
+template <int DH>
+constexpr int kValueRow = DH + 16; // halves per V row
+
+// channel at a position of an LDS row
+template <int DH>
+__device__ inline int channel_at(int position) {
+    const int unit = position >> 3;
+    const int group = unit < DH / 16 ? 2 * unit : 2 * (unit - DH / 16) + 1;
+    return 8 * group + (position & 7);
+}
 
 // Where a call's cached rows are; the same for every workgroup.
 struct CacheView {
@@ -77,6 +94,14 @@ __device__ inline bool piece_is_small(uint32_t scales) { // of the two groups of
     return scale_is_small(s2.x) && scale_is_small(s2.y);
 }
 
+// a piece on its way into LDS; row: the start of its row there, scales 0 for pieces past head_dim
+template <int DH>
+__device__ inline void stash_piece(half_t* row, int piece, const uint4_vt& q, uint32_t scales) {
+    const half2_t s2 = as_half2(scales);
+    *reinterpret_cast<half8_t*>(row + 8 * piece) = dequant8(q.x, q.y, s2.x);
+    *reinterpret_cast<half8_t*>(row + 8 * (DH / 16 + piece)) = dequant8(q.z, q.w, s2.y);
+}
+
 // Offset of a piece in a tile whose last existing row is `last`. Every lane loads something, without a branch: rows past
 // the last repeat it, pieces past head_dim repeat the first (their scales become zeros on the way into LDS). Token
 // strides are below 2^25 elements: 32 of them fit 32 bits.
@@ -88,7 +113,6 @@ template <int DH>
 struct CacheTile {
     static constexpr int PIECES = DH / 16; // 16-byte pieces of a row
     static constexpr int NLD = DH / 32; // pieces a lane loads
-    static constexpr int LDR = DH + 8; // halves per LDS row
     uint4_vt q[NLD];
     uint32_t s[NLD];
 
@@ -108,16 +132,14 @@ struct CacheTile {
         }
     }
 
-    __device__ inline void stash(half_t* tile, int head_dim) const {
+    // ldr: halves per LDS row (kKeyRow or kValueRow)
+    __device__ inline void stash(half_t* tile, int ldr, int head_dim) const {
         const int lane = threadIdx.x & 63;
 #pragma unroll
         for (int n = 0; n < NLD; ++n) {
             const uint32_t c = lane + 64 * n;
             const int row = c / PIECES, piece = c % PIECES;
-            const half2_t s2 = as_half2(16 * piece < head_dim ? s[n] : 0u);
-            half8_t* dst = reinterpret_cast<half8_t*>(tile + row * LDR + 16 * piece);
-            dst[0] = dequant8(q[n].x, q[n].y, s2.x);
-            dst[1] = dequant8(q[n].z, q[n].w, s2.y);
+            stash_piece<DH>(tile + row * ldr, piece, q[n], 16 * piece < head_dim ? s[n] : 0u);
         }
     }
 
@@ -132,11 +154,11 @@ struct CacheTile {
         return rows;
     }
     // as stash, with zeros for the pieces that may hold such values
-    __device__ inline void stash_finite(half_t* tile, int head_dim) const {
+    __device__ inline void stash_finite(half_t* tile, int ldr, int head_dim) const {
         CacheTile<DH> t = *this;
 #pragma unroll
         for (int n = 0; n < NLD; ++n) t.s[n] = piece_is_small(s[n]) ? s[n] : 0u;
-        t.stash(tile, head_dim);
+        t.stash(tile, ldr, head_dim);
     }
 };
 
@@ -146,7 +168,6 @@ struct SharedTile {
     static constexpr int PIECES = DH / 16;
     static constexpr int ALL = 2 * kTileKeys * PIECES; // K's, then V's
     static constexpr int NLD = (ALL + 64 * W - 1) / (64 * W);
-    static constexpr int LDR = DH + 8;
     uint4_vt q[NLD];
     uint32_t s[NLD];
 
@@ -171,23 +192,20 @@ struct SharedTile {
             s[n] = *reinterpret_cast<const uint32_t*>((const char*)v.scale + first / 4 + off / 4);
         }
     }
-    // odd: where to note the V rows with pieces that may not be finite (those become zeros); null: not looked at
-    __device__ inline void stash(half_t* k_tile, half_t* v_tile, int head_dim, uint32_t* odd) const {
+    // finite_values: V pieces that may not be finite become zeros; returns the rows of those this thread had
+    __device__ inline uint32_t stash(half_t* k_tile, half_t* v_tile, int head_dim, bool finite_values) const {
+        uint32_t odd = 0;
 #pragma unroll
         for (int n = 0; n < NLD; ++n) {
             int kv, row, piece;
             place(n, &kv, &row, &piece);
             if (row >= kTileKeys) break;
-            uint32_t sc = 16 * piece < head_dim ? s[n] : 0u;
-            if (odd && kv && !piece_is_small(sc)) {
-                sc = 0;
-                atomicOr(odd, 1u << row);
-            }
-            const half2_t s2 = as_half2(sc);
-            half8_t* dst = reinterpret_cast<half8_t*>((kv ? v_tile : k_tile) + row * LDR + 16 * piece);
-            dst[0] = dequant8(q[n].x, q[n].y, s2.x);
-            dst[1] = dequant8(q[n].z, q[n].w, s2.y);
+            const bool keep = !(finite_values && kv) || piece_is_small(s[n]);
+            odd |= keep ? 0u : 1u << row;
+            stash_piece<DH>(kv ? v_tile + row * kValueRow<DH> : k_tile + row * kKeyRow<DH>, piece, q[n],
+                            16 * piece < head_dim && keep ? s[n] : 0u);
         }
+        return odd;
     }
 };
 

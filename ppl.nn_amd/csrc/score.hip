@@ -33,7 +33,7 @@ constexpr int kScoreRows = 256; // rows whose log-sums are held in LDS at a time
 
 template <int DH>
 __global__ __launch_bounds__(256, 2) void kv_score_kernel(const ScoreParams p) {
-    constexpr int LDR = CacheTile<DH>::LDR;
+    constexpr int LDR = kKeyRow<DH>;
     constexpr int KC2 = DH / 32;
     __shared__ __attribute__((aligned(16))) half_t lds[4 * kTileKeys * LDR];
     __shared__ __attribute__((aligned(16))) float row_lse[kScoreRows]; // in units of log2
@@ -56,7 +56,7 @@ __global__ __launch_bounds__(256, 2) void kv_score_kernel(const ScoreParams p) {
     const int64_t key0 = block0 + wave * kScoreWaveKeys;
     half_t* const tile = lds + wave * kTileKeys * LDR;
 
-    // ---- the wave's keys as B operands: key 16 * kb + r_lane, channels 32 * kc + 8 * g .. + 7
+    // ---- the wave's keys as B operands: key 16 * kb + r_lane, positions 32 * kc + 8 * g .. + 7 of its LDS row
     half8_t kf[4][KC2];
     const bool have_keys = key0 < kvlen;
     if (have_keys) {
@@ -69,7 +69,7 @@ __global__ __launch_bounds__(256, 2) void kv_score_kernel(const ScoreParams p) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             wave_lds_order();
-            raw[h].stash(tile, hd);
+            raw[h].stash(tile, LDR, hd);
             wave_lds_order();
 #pragma unroll
             for (int i = 0; i < 2; ++i)
@@ -100,12 +100,13 @@ __global__ __launch_bounds__(256, 2) void kv_score_kernel(const ScoreParams p) {
         for (int r0 = 0; r0 < n; r0 += 16) {
             const int64_t row = chunk + r0 + r_lane < rows ? chunk + r0 + r_lane : rows - 1;
             const int64_t t = row / p.rep;
-            const half_t* qp = p.q + ((s0 + t) * p.num_heads + kvh * p.rep + (row - t * p.rep)) * hd + 8 * g;
+            const half_t* qp = p.q + ((s0 + t) * p.num_heads + kvh * p.rep + (row - t * p.rep)) * hd;
             half8_t qf[KC2];
 #pragma unroll
             for (int kc = 0; kc < KC2; ++kc) {
-                if (32 * kc + 8 * g < hd) {
-                    qf[kc] = *reinterpret_cast<const half8_t*>(qp + 32 * kc);
+                const int channel = channel_at<DH>(32 * kc + 8 * g);
+                if (channel < hd) {
+                    qf[kc] = *reinterpret_cast<const half8_t*>(qp + channel);
                 } else {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) qf[kc][e] = (half_t)0.f;

@@ -134,8 +134,15 @@ __device__ inline uint32_t visible_keys(const uint64_t* row_mask, int words, int
     return n >= 32 ? see : see & ((1u << n) - 1);
 }
 
+// A value the compiler must take as new: addresses formed from it in code behind or beside the tile loop are not computed
+// ahead of the loop and held in registers throughout.
+__device__ inline int recomputed(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
 // What a wave holds of its N blocks of 16 rows: lane (g = lane / 16, lane % 16) row lane % 16 of each block, of the output
-// channels 16 i + 4 g .. + 3 and of the sum its own keys' share.
+// positions 16 i + 4 g .. + 3 (channel_at) and of the sum its own keys' share.
 template <int DH, int N>
 struct RowState {
     int tok[N]; // token of the sequence; -1 for rows past the last one
@@ -153,8 +160,10 @@ struct RowState {
             tok[n] = row < rows ? t : -1;
             const half_t* qp = p.q + ((s0 + t) * p.num_heads + kvh * p.rep + (rr - t * p.rep)) * p.view.head_dim;
 #pragma unroll
-            for (int kc = 0; kc < DH / 32; ++kc) // (groups past head_dim: the first one, zeroed in queries_here)
-                qf[n][kc] = *reinterpret_cast<const half8_t*>(qp + (32 * kc + 8 * g < p.view.head_dim ? 32 * kc + 8 * g : 0));
+            for (int kc = 0; kc < DH / 32; ++kc) { // (groups past head_dim: the first one, zeroed in queries_here)
+                const int channel = channel_at<DH>(32 * kc + 8 * g);
+                qf[n][kc] = *reinterpret_cast<const half8_t*>(qp + (channel < p.view.head_dim ? channel : 0));
+            }
             m[n] = -INFINITY;
             shift[n] = kProbShift;
             l[n] = 0.f;
@@ -172,26 +181,34 @@ struct RowState {
 #pragma unroll
             for (int kc = 0; kc < DH / 32; ++kc) {
                 asm volatile("" : "+v"(qf[n][kc]));
-                if (head_dim < DH && 32 * kc + 8 * g >= head_dim) qf[n][kc] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
+                if (head_dim < DH && channel_at<DH>(32 * kc + 8 * g) >= head_dim) qf[n][kc] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
             }
         }
     }
 
-    // scores of the rows against the 32 keys in `tile`: s[n][tb][e] belongs to key 16 * tb + 4 * g + e
-    __device__ inline void scores(const half_t* tile, float (&s)[N][2][4]) const {
+    // the 32 keys in `tile` as operands: keys 16 * tb + lane % 16, positions 32 * kc + 8 * g .. + 7
+    typedef half8_t KeyOperands[2][DH / 32];
+    __device__ static inline void load_keys(const half_t* tile, KeyOperands& kf) {
         const int lane = threadIdx.x & 63, g = lane >> 4;
+#pragma unroll
+        for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+            for (int kc = 0; kc < DH / 32; ++kc)
+                kf[tb][kc] = *reinterpret_cast<const half8_t*>(tile + (16 * tb + (lane & 15)) * kKeyRow<DH> + 32 * kc + 8 * g);
+    }
+
+    // scores of the rows against those keys: s[n][tb][e] belongs to key 16 * tb + 4 * g + e
+    __device__ inline void scores(const KeyOperands& kf, float (&s)[N][2][4]) const {
 #pragma unroll
         for (int tb = 0; tb < 2; ++tb) {
             float4_t acc[N];
 #pragma unroll
             for (int n = 0; n < N; ++n) acc[n] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int kc = 0; kc < DH / 32; ++kc) {
-                const half8_t a = *reinterpret_cast<const half8_t*>(tile + (16 * tb + (lane & 15)) * CacheTile<DH>::LDR +
-                                                                    32 * kc + 8 * g);
+            for (int kc = 0; kc < DH / 32; ++kc)
 #pragma unroll
-                for (int n = 0; n < N; ++n) acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qf[n][kc], acc[n], 0, 0, 0);
-            }
+                for (int n = 0; n < N; ++n)
+                    acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[tb][kc], qf[n][kc], acc[n], 0, 0, 0);
 #pragma unroll
             for (int n = 0; n < N; ++n)
 #pragma unroll
@@ -216,16 +233,16 @@ struct RowState {
         }
     }
 
-    // scores -> weights (fp16, the operand of the second product), running sums
-    __device__ inline void weights(float scale_log2, const float (&s)[N][2][4], half8_t (&pp)[N]) {
+    // moves a row's reference point where a score passes it by too much
+    __device__ inline void settle(float scale_log2, const float (&s)[N][2][4]) {
         float top[N];
         bool moves = false;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             top[n] = fmaxf(fmaxf(fmaxf(s[n][0][0], s[n][0][1]), fmaxf(s[n][0][2], s[n][0][3])),
                            fmaxf(fmaxf(s[n][1][0], s[n][1][1]), fmaxf(s[n][1][2], s[n][1][3])));
-            moves = moves || __builtin_fmaf(top[n], scale_log2, shift[n]) > kProbShift + kSlack ||
-                    (m[n] == -INFINITY && top[n] > -INFINITY);
+            moves |= (__builtin_fmaf(top[n], scale_log2, shift[n]) > kProbShift + kSlack) |
+                     ((m[n] == -INFINITY) & (top[n] > -INFINITY));
         }
         if (__any(moves)) { // (rows without a key so far keep m = -inf: weights exp2(-inf) = 0)
 #pragma unroll
@@ -240,6 +257,10 @@ struct RowState {
                 for (int i = 0; i < DH / 16; ++i) o[n][i] *= alpha;
             }
         }
+    }
+
+    // scores -> weights (fp16, the operand of the second product) and their sums
+    __device__ inline void weights(float scale_log2, const float (&s)[N][2][4], half8_t (&pp)[N]) {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             float sum = 0.f;
@@ -255,31 +276,37 @@ struct RowState {
         }
     }
 
-    // o += weights x the 32 value rows in `tile`
-    __device__ inline void values(const half_t* tile, const half8_t (&pp)[N]) {
-        constexpr int LDR = CacheTile<DH>::LDR;
+    // the 32 value rows in `tile`, transposed: lane (g, j) gets position 16 * i + j of keys 4 * g .. + 3 and 16 + 4 * g .. + 3
+    typedef half8_t ValueOperands[DH / 16];
+    __device__ static inline void load_values(const half_t* tile, ValueOperands& vf) {
+        constexpr int LDR = kValueRow<DH>;
         const int lane = threadIdx.x & 63, g = lane >> 4, j = lane & 15;
 #pragma unroll
         for (int i = 0; i < DH / 16; ++i) {
-            // lane (g, j) receives channel 16 * i + j of keys 4 * g .. + 3 and 16 + 4 * g .. + 3
             const half_t* src = tile + (4 * g + (j >> 2)) * LDR + 16 * i + 4 * (j & 3);
             const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)src);
             const short4_t hi =
                 __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)(src + 16 * LDR));
-            half8_t a;
-            __builtin_memcpy(&a, &lo, 8);
-            __builtin_memcpy(reinterpret_cast<char*>(&a) + 8, &hi, 8);
-#pragma unroll
-            for (int n = 0; n < N; ++n) o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pp[n], o[n][i], 0, 0, 0);
+            __builtin_memcpy(&vf[i], &lo, 8);
+            __builtin_memcpy(reinterpret_cast<char*>(&vf[i]) + 8, &hi, 8);
         }
     }
 
-    // Value pieces that may not be finite are zeros in the tile (a key can be hidden from a row: its weight there is 0,
-    // and 0 times a NaN or an infinity is NaN). Here they are multiplied key by key, and the result is taken over by the
-    // rows that see the key only. rows: which rows of the tile have such pieces; base: offset of its first V row.
+    // o += weights x those rows
+    __device__ inline void values(const ValueOperands& vf, const half8_t (&pp)[N]) {
+#pragma unroll
+        for (int i = 0; i < DH / 16; ++i)
+#pragma unroll
+            for (int n = 0; n < N; ++n) o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[i], pp[n], o[n][i], 0, 0, 0);
+    }
+
+    // Value pieces that may not be finite are zeros in the tiles (a key can be hidden from a row: its weight there is 0,
+    // and 0 times a NaN or an infinity is NaN). Once a piece's tiles are done, those that had such pieces are gone through
+    // again: here they are multiplied key by key, and the result is taken over by the rows that see the key only. rows:
+    // which rows of the tile have such pieces; base: offset of its first V row.
     __device__ inline void odd_values(const TreeParams& p, int64_t base, int kv0, int kvlen, uint32_t rows,
                                       const half8_t (&pp)[N], const uint32_t (&see)[N]) {
-        const int lane = threadIdx.x & 63, g = lane >> 4;
+        const int lane = recomputed(threadIdx.x & 63), g = lane >> 4;
 #pragma unroll 1
         for (; rows; rows &= rows - 1) {
             const int row = __builtin_ctz(rows);
@@ -290,9 +317,10 @@ struct RowState {
 #pragma unroll
             for (int i = 0; i < DH / 16; ++i) {
                 __builtin_amdgcn_sched_barrier(0);
-                if (16 * i >= p.view.head_dim || (scale_is_small(vs[2 * i]) && scale_is_small(vs[2 * i + 1]))) continue;
-                const int d = 16 * i + (lane & 15);
-                const half_t v = (half_t)((float)vq[d] * (float)vs[d >> 3]);
+                const int d = channel_at<DH>(16 * i + (lane & 15));
+                half_t v = (half_t)0.f;
+                if (d < p.view.head_dim && !(scale_is_small(vs[d >> 4 << 1]) && scale_is_small(vs[(d >> 4 << 1) + 1])))
+                    v = (half_t)((float)vq[d] * (float)vs[d >> 3]);
                 half8_t a;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) a[e] = g == ((row >> 2) & 3) && e == slot ? v : (half_t)0.f;
@@ -314,7 +342,7 @@ __device__ inline void finish_row(const TreeParams& p, int64_t s0, int row, int 
     const int64_t at = (s0 + t) * p.num_heads + kvh * p.rep + (row - t * p.rep);
     const float inv = l != 0.f ? 1.0f / l : 0.f;
     const half4_t r = {(half_t)(a[0] * inv), (half_t)(a[1] * inv), (half_t)(a[2] * inv), (half_t)(a[3] * inv)};
-    *reinterpret_cast<half4_t*>(p.out + at * p.view.head_dim + d) = r;
+    if (d < p.view.head_dim) *reinterpret_cast<half4_t*>(p.out + at * p.view.head_dim + d) = r;
     if (p.lse && d == 0) p.lse[at] = l == 0.f ? -INFINITY : (m_log2 + (log2f(l) - kProbShift)) * 0.693147180559945f;
 }
 
@@ -393,15 +421,13 @@ constexpr int tree_waves_per_simd(int dh, int row_blocks) {
 template <int DH, int NR>
 __global__ __launch_bounds__(256, tree_waves_per_simd(DH, NR)) void tree_keys_kernel(const TreeParams p) {
     constexpr int ROWS = 16 * NR;
-    constexpr int LDR = CacheTile<DH>::LDR;
+    constexpr int LDR = kValueRow<DH>; // (of the region: a K tile takes a little less)
     constexpr int LDO = DH + 4; // floats per row of the combination
     static_assert(kTreeWaves * kTileKeys * LDR * 2 >= kTreeWaves * 16 * LDO * 4, "the combination reuses the tiles");
     __shared__ __attribute__((aligned(16))) half_t lds[kTreeWaves * kTileKeys * LDR];
     __shared__ float2 ml_lds[kTreeWaves][ROWS];
 
-    const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int r_lane = lane & 15, g = lane >> 4;
     const int range = blockIdx.x / p.kv_heads;
     const int kvh = blockIdx.x - range * p.kv_heads;
     half_t* const tile = lds + wave * kTileKeys * LDR;
@@ -416,7 +442,8 @@ __global__ __launch_bounds__(256, tree_waves_per_simd(DH, NR)) void tree_keys_ke
         CacheTile<DH> rk, rv; // the next tile's K and V rows, on their way
         int kt = t.key_tile + wave;
         const int first_key = (kt < t.stop_tile ? kt : t.key_tile) * kTileKeys; // (a wave without a tile: any)
-        int64_t base = p.view.key_row(t.b, first_key, kvh), base_now = base;
+        int64_t base = p.view.key_row(t.b, first_key, kvh);
+        bool odd_tiles = false;
         rk.fetch(p.view, base, first_key, t.kvlen);
         rv.fetch(p.view, base + p.view.addr.stride_kv, first_key, t.kvlen);
         st.queries_here(p.view.head_dim);
@@ -424,32 +451,63 @@ __global__ __launch_bounds__(256, tree_waves_per_simd(DH, NR)) void tree_keys_ke
             const int kv0 = kt * kTileKeys;
             const int kv_next = kt + kTreeWaves < t.stop_tile ? kv0 + kTreeWaves * kTileKeys : kv0; // (the last: again)
             const bool history = kv0 + kTileKeys <= t.start; // every row sees every key
-            base_now = base;
             wave_lds_order();
-            rk.stash(tile, p.view.head_dim);
+            rk.stash(tile, kKeyRow<DH>, p.view.head_dim);
             wave_lds_order();
             base = p.view.key_row(t.b, kv_next, kvh);
             rk.fetch(p.view, base, kv_next, t.kvlen);
             float s[NR][2][4];
             uint32_t see[NR];
             half8_t pp[NR];
-            st.scores(tile, s);
+            typename RowState<DH, NR>::KeyOperands kf;
+            typename RowState<DH, NR>::ValueOperands vf;
+            st.load_keys(tile, kf);
+            st.scores(kf, s);
             if (!history) st.hide(p, t.s0, kv0, t.start, t.kvlen, s, see);
+            st.settle(p.scale_log2, s);
             st.weights(p.scale_log2, s, pp);
-            const uint32_t odd = history ? 0u : rv.odd_rows();
             wave_lds_order();
-            if (odd)
-                rv.stash_finite(tile, p.view.head_dim);
-            else
-                rv.stash(tile, p.view.head_dim);
+            if (!history && rv.odd_rows()) {
+                odd_tiles = true;
+                rv.stash_finite(tile, kValueRow<DH>, p.view.head_dim);
+            } else {
+                rv.stash(tile, kValueRow<DH>, p.view.head_dim);
+            }
             wave_lds_order();
             rv.fetch(p.view, base + p.view.addr.stride_kv, kv_next, t.kvlen);
-            st.values(tile, pp);
-            if (odd) st.odd_values(p, base_now + p.view.addr.stride_kv, kv0, t.kvlen, odd, pp, see);
+            st.load_values(tile, vf);
+            st.values(vf, pp);
+        }
+        if (odd_tiles) {
+            float l_done[NR];
+#pragma unroll
+            for (int n = 0; n < NR; ++n) l_done[n] = st.l[n];
+            for (kt = t.key_tile + wave; kt < t.stop_tile; kt += kTreeWaves) {
+                const int kv0 = kt * kTileKeys;
+                if (kv0 + kTileKeys <= t.start) continue;
+                base = p.view.key_row(t.b, kv0, kvh);
+                rk.fetch(p.view, base, kv0, t.kvlen);
+                rv.fetch(p.view, base + p.view.addr.stride_kv, kv0, t.kvlen);
+                wave_lds_order();
+                rk.stash(tile, kKeyRow<DH>, p.view.head_dim);
+                wave_lds_order();
+                float s[NR][2][4];
+                uint32_t see[NR];
+                half8_t pp[NR];
+                typename RowState<DH, NR>::KeyOperands kf;
+                st.load_keys(tile, kf);
+                st.scores(kf, s);
+                st.hide(p, t.s0, kv0, t.start, t.kvlen, s, see);
+                st.weights(p.scale_log2, s, pp);
+                st.odd_values(p, base + p.view.addr.stride_kv, kv0, t.kvlen, rv.odd_rows(), pp, see);
+            }
+#pragma unroll
+            for (int n = 0; n < NR; ++n) st.l[n] = l_done[n]; // (the sums were complete)
         }
 
         // ---- the four waves' shares of the piece, joined 16 rows at a time
         __syncthreads(); // (the tiles are read no more; the piece before has been written out)
+        const int tid = recomputed(threadIdx.x), r_lane = tid & 15, g = (tid & 63) >> 4;
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
             const float l = sum_over_groups(st.l[n]);
@@ -467,7 +525,7 @@ __global__ __launch_bounds__(256, tree_waves_per_simd(DH, NR)) void tree_keys_ke
             for (int i = 0; i < DH / 16; ++i)
                 *reinterpret_cast<float4_t*>(olds + (wave * 16 + r_lane) * LDO + 16 * i + 4 * g) = st.o[n][i] * f;
             __syncthreads();
-            for (int x = threadIdx.x; x < 16 * (DH / 4); x += 256) {
+            for (int x = tid; x < 16 * (DH / 4); x += 256) {
                 const int r = x / (DH / 4), d = (x - r * (DH / 4)) * 4;
                 float mm = -INFINITY;
                 for (int w = 0; w < kTreeWaves; ++w) mm = fmaxf(mm, ml_lds[w][16 * n + r].x);
@@ -480,7 +538,7 @@ __global__ __launch_bounds__(256, tree_waves_per_simd(DH, NR)) void tree_keys_ke
                 }
                 const int row = t.row0 + 16 * n + r;
                 if (t.whole) {
-                    if (row < t.rows && d < p.view.head_dim) finish_row(p, t.s0, row, kvh, d, a, mm, l);
+                    if (row < t.rows) finish_row(p, t.s0, row, kvh, channel_at<DH>(d), a, mm, l);
                 } else {
                     const int64_t at = t.slot * ROWS + 16 * n + r;
                     *reinterpret_cast<float4_t*>(p.part_o + at * DH + d) = a;
@@ -493,18 +551,15 @@ __global__ __launch_bounds__(256, tree_waves_per_simd(DH, NR)) void tree_keys_ke
 }
 
 // W waves, each with NB blocks of 16 rows: row block i of the tile is block i / W of wave i % W, so that few rows still
-// spread over all waves. The workgroup's threads bring a key tile's K and V pieces into one of two LDS buffers while the
-// other is computed on: one barrier per tile.
+// spread over all waves. The workgroup's threads bring the key tiles into LDS, two buffers and one barrier per tile.
 template <int DH, int W, int NB>
 __global__ __launch_bounds__(W * 64, tree_waves_per_simd(DH, NB)) void tree_rows_kernel(const TreeParams p) {
     constexpr int ROWS = 16 * W * NB;
-    constexpr int LDR = CacheTile<DH>::LDR;
-    __shared__ __attribute__((aligned(16))) half_t lds[2][2][kTileKeys * LDR]; // [buffer][K, V]
-    __shared__ uint32_t odd_lds[3]; // tile i's value rows that were kept out, in entry i % 3
+    __shared__ __attribute__((aligned(16))) half_t k_lds[2][kTileKeys * kKeyRow<DH>];
+    __shared__ __attribute__((aligned(16))) half_t v_lds[2][kTileKeys * kValueRow<DH>];
+    __shared__ uint32_t odd_lds; // value rows that were kept out of the tiles
 
-    const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int g = lane >> 4;
     const int range = blockIdx.x / p.kv_heads;
     const int kvh = blockIdx.x - range * p.kv_heads;
 
@@ -523,12 +578,14 @@ __global__ __launch_bounds__(W * 64, tree_waves_per_simd(DH, NB)) void tree_rows
             const int kv0 = (t.key_tile + (i < n_tiles ? i : n_tiles - 1)) * kTileKeys;
             r.fetch(p.view, p.view.key_row(t.b, kv0, kvh), kv0, t.kvlen);
         };
+        bool odd_pieces = false; // this thread has kept value pieces out of the tiles
         auto stash = [&](const SharedTile<DH, W>& r, int i) {
             const bool history = (t.key_tile + i + 1) * kTileKeys <= t.start;
-            r.stash(lds[i & 1][0], lds[i & 1][1], p.view.head_dim, history ? nullptr : &odd_lds[i % 3]);
+            odd_pieces |= r.stash(k_lds[i & 1], v_lds[i & 1], p.view.head_dim, !history) != 0;
         };
+        uint32_t see[NB];
         __syncthreads(); // (the piece before has read its last tile)
-        if (threadIdx.x < 3) odd_lds[threadIdx.x] = 0;
+        if (threadIdx.x == 0) odd_lds = 0;
         if (n_tiles > 0) {
             fetch(raw[0], 0);
             fetch(raw[1], 1);
@@ -541,26 +598,37 @@ __global__ __launch_bounds__(W * 64, tree_waves_per_simd(DH, NB)) void tree_rows
         }
         __syncthreads();
         auto step = [&](SharedTile<DH, W>& next, int i) { // next: tile i + 1, then tile i + 3
-            if (threadIdx.x == 0) odd_lds[(i + 2) % 3] = 0;
-            if (busy) {
-                const int kv0 = (t.key_tile + i) * kTileKeys;
-                const bool history = kv0 + kTileKeys <= t.start;
-                float s[NB][2][4];
-                uint32_t see[NB];
-                half8_t pp[NB];
-                st.scores(lds[i & 1][0], s);
-                if (!history) st.hide(p, t.s0, kv0, t.start, t.kvlen, s, see);
-                st.weights(p.scale_log2, s, pp);
-                st.values(lds[i & 1][1], pp);
-                const uint32_t odd = history ? 0u : __builtin_amdgcn_readfirstlane(odd_lds[i % 3]);
-                if (odd)
-                    st.odd_values(p, p.view.key_row(t.b, kv0, kvh) + p.view.addr.stride_kv, kv0, t.kvlen, odd, pp, see);
-            }
-            stash(next, i + 1); // (past the last tile: into the buffer nobody reads any more)
+            const int kv0 = (t.key_tile + i) * kTileKeys;
+            float s[NB][2][4];
+            half8_t pp[NB];
+            typename RowState<DH, NB>::KeyOperands kf;
+            typename RowState<DH, NB>::ValueOperands vf;
+            st.load_keys(k_lds[i & 1], kf);
+            __builtin_amdgcn_sched_barrier(0); // (the keys come out of LDS while the next tile goes in ..)
+            stash(next, i + 1);
             fetch(next, i + 3);
+            st.scores(kf, s);
+            __builtin_amdgcn_sched_barrier(0);
+            st.load_values(v_lds[i & 1], vf); // (.. and the values, into the keys' registers, while the weights are formed)
+            __builtin_amdgcn_sched_barrier(0);
+            if (kv0 + kTileKeys > t.start) st.hide(p, t.s0, kv0, t.start, t.kvlen, s, see);
+            st.settle(p.scale_log2, s);
+            st.weights(p.scale_log2, s, pp);
+            st.values(vf, pp);
             __syncthreads();
         };
-        if (n_tiles > 0) {
+        if (!busy) { // the same stashes, fetches and barriers as the others'
+            for (int i = 0; i < n_tiles; ++i) {
+                if (i & 1) {
+                    stash(raw[0], i + 1);
+                    fetch(raw[0], i + 3);
+                } else {
+                    stash(raw[1], i + 1);
+                    fetch(raw[1], i + 3);
+                }
+                __syncthreads();
+            }
+        } else if (n_tiles > 0) {
             for (int i = 0;;) { // (left from the middle, so that at its head raw[1] is always the older of the two)
                 step(raw[1], i);
                 if (++i >= n_tiles) break;
@@ -568,6 +636,37 @@ __global__ __launch_bounds__(W * 64, tree_waves_per_simd(DH, NB)) void tree_rows
                 if (++i >= n_tiles) break;
             }
         }
+        if (odd_pieces) odd_lds = 1;
+        __syncthreads();
+        if (odd_lds) {
+            float l_done[NB];
+#pragma unroll
+            for (int n = 0; n < NB; ++n) l_done[n] = st.l[n];
+            for (int i = 0; i < n_tiles; ++i) {
+                const int kv0 = (t.key_tile + i) * kTileKeys;
+                if (kv0 + kTileKeys <= t.start) continue;
+                fetch(raw[0], i);
+                __syncthreads(); // everybody has read the tile before, and odd_lds
+                if (threadIdx.x == 0) odd_lds = 0;
+                __syncthreads();
+                const uint32_t odd = raw[0].stash(k_lds[0], v_lds[0], p.view.head_dim, true);
+                if (odd) atomicOr(&odd_lds, odd);
+                __syncthreads();
+                if (!busy) continue;
+                float s[NB][2][4];
+                half8_t pp[NB];
+                typename RowState<DH, NB>::KeyOperands kf;
+                st.load_keys(k_lds[0], kf);
+                st.scores(kf, s);
+                st.hide(p, t.s0, kv0, t.start, t.kvlen, s, see);
+                st.weights(p.scale_log2, s, pp);
+                st.odd_values(p, p.view.key_row(t.b, kv0, kvh) + p.view.addr.stride_kv, kv0, t.kvlen,
+                              __builtin_amdgcn_readfirstlane(odd_lds), pp, see);
+            }
+#pragma unroll
+            for (int n = 0; n < NB; ++n) st.l[n] = l_done[n]; // (the sums were complete)
+        }
+        const int lane = recomputed(threadIdx.x & 63), g = lane >> 4;
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
             const float l = sum_over_groups(st.l[n]);
@@ -575,8 +674,9 @@ __global__ __launch_bounds__(W * 64, tree_waves_per_simd(DH, NB)) void tree_rows
             if (t.whole) {
 #pragma unroll
                 for (int i = 0; i < DH / 16; ++i)
-                    if (st.tok[n] >= 0 && 16 * i < p.view.head_dim)
-                        finish_row(p, t.s0, t.row0 + r, kvh, 16 * i + 4 * g, st.o[n][i], st.m[n] * p.scale_log2, l);
+                    if (st.tok[n] >= 0)
+                        finish_row(p, t.s0, t.row0 + r, kvh, channel_at<DH>(16 * i + 4 * g), st.o[n][i],
+                                   st.m[n] * p.scale_log2, l);
             } else if (st.tok[n] >= 0) {
                 const int64_t at = t.slot * ROWS + r;
 #pragma unroll
@@ -607,7 +707,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeParams p, con
     for (int x = blockIdx.y * 256 + threadIdx.x; x < ROWS * (DH / 4); x += 256 * gridDim.y) {
         const int r = x / (DH / 4), d = (x - r * (DH / 4)) * 4;
         const int row = (int)row_tile * ROWS + r;
-        if (row >= rows || d >= p.view.head_dim) continue;
+        if (row >= rows) continue;
         float m = -INFINITY, l = 0.f;
         float4_t a = {0.f, 0.f, 0.f, 0.f};
         for (int k = range - 1; k <= last; ++k) {
@@ -621,7 +721,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeParams p, con
             a = a * fo + v * fn;
             m = m_new;
         }
-        finish_row(p, s0, row, kvh, d, a, m, l);
+        finish_row(p, s0, row, kvh, channel_at<DH>(d), a, m, l);
     }
 }
 
