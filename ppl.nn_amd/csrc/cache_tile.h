@@ -22,6 +22,13 @@ typedef const int64_t __attribute__((address_space(4)))* const_tab64_t; // wave-
 
 constexpr int kTileKeys = 32;
 
+// PageMap::token for a wave-uniform (b, j): scalar loads, whatever the kernel has stored before
+__device__ inline int64_t uniform_token(const PageMap& pages, int b, int j) {
+    const const_tab64_t tab = (const_tab64_t)pages.cachestarts;
+    if (pages.page_shift == 0) return tab[b] + j;
+    return tab[b * pages.stride_b + (j >> pages.page_shift)] + (j & ((1 << pages.page_shift) - 1));
+}
+
 template <int DH>
 constexpr int kKeyRow = DH + 8; // halves per K row in LDS
 template <int DH>
@@ -39,19 +46,14 @@ __device__ inline int channel_at(int position) {
 struct CacheView {
     const int8_t* cache;
     const half_t* scale;
-    const int64_t* cachestarts;
-    int64_t cs_stride_b;
+    PageMap pages;
     CacheAddr addr;
-    int32_t page_shift; // 0: contiguous region per sequence
     int32_t head_dim;
 
     // element offset of the K row of key j of sequence b (both wave-uniform; a run of 32 keys from a multiple of 32
     // lies in one page: pages are powers of two of at least 64 tokens)
     __device__ inline int64_t key_row(int b, int j, int kvh) const {
-        const const_tab64_t tab = (const_tab64_t)cachestarts;
-        const int64_t t = page_shift == 0 ? tab[b] + j
-                                          : tab[b * cs_stride_b + (j >> page_shift)] + (j & ((1 << page_shift) - 1));
-        return addr.row(t, 0, kvh);
+        return addr.row(uniform_token(pages, b, j), 0, kvh);
     }
 };
 

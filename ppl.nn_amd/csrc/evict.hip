@@ -5,10 +5,11 @@
 // the first K places move, each into the place of a row in front that goes: as few row moves as possible, and sources
 // (index >= K) and destinations (index < K) never overlap, so all of them run in parallel, in place.
 //
-// kv_evict_choose_kernel: one workgroup per (sequence, layer, kv head). The K-th largest key is found digit by digit (8
-// bits at a time, counts in LDS), then one more pass in index order numbers the holes and the rows that fill them.
+// kv_evict_choose_kernel: one workgroup per (sequence, layer, kv head). It reads the scores and positions once, as sort keys
+// into registers (up to 64 a thread), finds the K-th largest digit by digit (8 bits at a time, counts in LDS), then
+// numbers, in index order, the holes and the rows that fill them.
 // kv_evict_move_kernel: 16-byte pieces of the listed rows, K and V, with their scales.
-#include "common.h"
+#include "cache_tile.h"
 
 namespace pplhip {
 
@@ -35,10 +36,6 @@ struct EvictParams {
     int32_t* fills; // .. and of the row that goes there
 };
 
-constexpr int kChooseThreads = 512;
-constexpr int kChooseWaves = kChooseThreads / 64;
-constexpr int kHistCopies = 16; // copies of the digit counts: scores share their leading bits, so lanes would queue
-
 struct EvictColumn {
     int32_t b, layer, head;
     int64_t scores; // offset of the column in the score and position arrays
@@ -61,13 +58,28 @@ __device__ inline uint32_t evict_key(const EvictParams& p, float score, int32_t 
     return u >> 31 ? ~u : u | 0x80000000u;
 }
 
-__global__ __launch_bounds__(kChooseThreads) void kv_evict_choose_kernel(const EvictParams p) {
-    __shared__ uint32_t hist[256 * kHistCopies];
-    __shared__ uint32_t wave_sum[kChooseWaves];
-    __shared__ uint32_t found[2]; // digit, rows above it
-    __shared__ int32_t seg_gt[kChooseWaves], seg_eq[kChooseWaves];
+// set bits of a wave-wide mask at the lanes below this one
+__device__ inline int lanes_below(uint64_t mask) {
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+}
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+// A column's tokens in blocks of T * KEYS, wave w of the block its w-th stretch: 64 consecutive tokens per key register, so
+// that loads are coalesced, index order is (block, wave, register, lane), and the 64 tokens lie in one page. A column of
+// one block (T * KEYS covers it) is loaded once; a longer one anew for each of the six looks at it.
+template <int T, int KEYS>
+__global__ __launch_bounds__(T) void kv_evict_choose_kernel(const EvictParams p) {
+    constexpr int WAVES = T / 64;
+    // copies of the digit counts: scores share their leading bits, so lanes would queue at one counter; few keys do not
+    // pay for clearing and adding up many
+    constexpr int kHistCopies = T * KEYS > 4096 ? 16 : 4;
+    constexpr int kBatch = KEYS < 16 ? KEYS : 16; // tokens whose loads a thread has in flight
+    __shared__ uint32_t hist[256 * kHistCopies];
+    __shared__ uint32_t wave_sum[4];
+    __shared__ uint32_t found[2]; // digit, rows above it
+    __shared__ int32_t seg_gt[WAVES], seg_eq[WAVES];
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const EvictColumn col = evict_column(p, blockIdx.x);
     const int64_t kvlen64 = p.kvstarts[col.b + 1] - p.kvstarts[col.b];
     const int64_t want = p.target[col.b] < 0 ? 0 : p.target[col.b];
@@ -78,33 +90,60 @@ __global__ __launch_bounds__(kChooseThreads) void kv_evict_choose_kernel(const E
     const bool copy_score = p.score_out != p.score_in, copy_pos = p.pos_in && p.pos_out != p.pos_in;
     if (keep == n || keep == 0) { // nothing moves
         if (tid == 0) p.moves[blockIdx.x] = 0;
-        for (int j = tid; j < keep; j += kChooseThreads) {
-            const int64_t at = col.scores + p.pages.token(col.b, j);
-            if (copy_score) p.score_out[at] = p.score_in[at];
-            if (copy_pos) p.pos_out[at] = p.pos_in[at];
-        }
+        if (copy_score || copy_pos)
+            for (int j = tid; j < keep; j += T) {
+                const int64_t at = col.scores + p.pages.token(col.b, j);
+                if (copy_score) p.score_out[at] = p.score_in[at];
+                if (copy_pos) p.pos_out[at] = p.pos_in[at];
+            }
         return;
     }
-    auto key_of = [&](int j) {
-        const int64_t at = col.scores + p.pages.token(col.b, j);
-        return evict_key(p, p.score_in[at], p.pos_in ? p.pos_in[at] : 0, next);
+    const int blocks = (n + T * KEYS - 1) / (T * KEYS);
+    const int regs = blocks > 1 ? KEYS : (n + T - 1) / T; // registers in use
+    uint32_t key[KEYS];
+    // first token of the wave's register k in a block
+    auto first_of = [&](int block, int k) { return block * (T * KEYS) + (wave * regs + k) * 64; };
+    auto load = [&](int block) {
+#pragma unroll
+        for (int k0 = 0; k0 < KEYS; k0 += kBatch) {
+            float score[kBatch];
+            int32_t pos[kBatch];
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                const int j = first_of(block, k0 + k);
+                score[k] = NAN; // past the end: the smallest key, behind all others of its kind
+                pos[k] = p.num_sink;
+                if (k0 + k < regs && j + lane < n) {
+                    const int64_t at = col.scores + uniform_token(p.pages, col.b, j) + lane;
+                    score[k] = p.score_in[at];
+                    if (p.pos_in) pos[k] = p.pos_in[at];
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k)
+                key[k0 + k] = first_of(block, k0 + k) + lane < n ? evict_key(p, score[k], pos[k], next) : 0u;
+        }
     };
+    if (blocks == 1) load(0);
 
     // ---- the keep-th largest key: `prefix` collects its digits, `remain` counts rows still to be found below them
     uint32_t prefix = 0;
     uint32_t remain = (uint32_t)keep;
     for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int i = tid; i < 256 * kHistCopies; i += kChooseThreads) hist[i] = 0;
+        for (int i = tid; i < 256 * kHistCopies; i += T) hist[i] = 0;
         __syncthreads();
-        for (int j = tid; j < n; j += kChooseThreads) {
-            const uint32_t k = key_of(j);
-            if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8)))
-                atomicAdd(&hist[((k >> shift) & 255) * kHistCopies + (lane & (kHistCopies - 1))], 1u);
+        for (int block = 0; block < blocks; ++block) {
+            if (blocks > 1) load(block);
+#pragma unroll
+            for (int k = 0; k < KEYS; ++k)
+                if (k < regs && (shift == 24 || (key[k] >> (shift + 8)) == (prefix >> (shift + 8))))
+                    atomicAdd(&hist[((key[k] >> shift) & 255) * kHistCopies + (lane & (kHistCopies - 1))], 1u);
         }
         __syncthreads();
         uint32_t mine = 0, incl = 0;
         if (tid < 256) { // thread i: digit 255 - i, so that the running sum counts from the largest digit down
-            for (int c = 0; c < kHistCopies; ++c) mine += hist[(255 - tid) * kHistCopies + c];
+#pragma unroll
+            for (int c = 0; c < kHistCopies; ++c) mine += hist[(255 - tid) * kHistCopies + ((c + tid) & (kHistCopies - 1))];
             incl = mine;
             for (int d = 1; d < 64; d <<= 1) {
                 const uint32_t up = __shfl_up(incl, d);
@@ -123,80 +162,127 @@ __global__ __launch_bounds__(kChooseThreads) void kv_evict_choose_kernel(const E
         __syncthreads();
         prefix |= found[0] << shift;
         remain -= found[1];
-        __syncthreads();
     }
     const int need_equal = (int)remain; // rows with exactly this key that stay: the first ones
 
-    // ---- in index order: every wave counts its own stretch, then numbers the rows in it
-    const int stretch = ((n + kChooseThreads - 1) / kChooseThreads) * 64;
-    const int j0 = wave * stretch, j1 = j0 + stretch < n ? j0 + stretch : n;
-    int gt = 0, eq = 0;
-    for (int j = j0; j < j1; j += 64) {
-        const bool in = j + lane < j1;
-        const uint32_t k = in ? key_of(j + lane) : 0;
-        gt += __popcll(__ballot(in && k > prefix));
-        eq += __popcll(__ballot(in && k == prefix));
-    }
-    if (lane == 0) {
-        seg_gt[wave] = gt;
-        seg_eq[wave] = eq;
-    }
-    __syncthreads();
-    int gt_before = 0, eq_before = 0;
-    for (int w = 0; w < wave; ++w) {
-        gt_before += seg_gt[w];
-        eq_before += seg_eq[w];
-    }
+    // ---- in index order: every wave counts its stretch, then numbers the rows in it
     int32_t* const holes = p.holes + (int64_t)blockIdx.x * p.max_moves;
     int32_t* const fills = p.fills + (int64_t)blockIdx.x * p.max_moves;
-    const uint64_t below = (uint64_t(1) << lane) - 1;
-    for (int j = j0; j < j1; j += 64) {
-        const int i = j + lane;
-        const bool in = i < j1;
-        const int64_t at = col.scores + p.pages.token(col.b, in ? i : j);
-        const float score = p.score_in[at];
-        const int32_t pos = p.pos_in ? p.pos_in[at] : 0;
-        const uint32_t k = evict_key(p, score, pos, next);
-        const uint64_t gts = __ballot(in && k > prefix), eqs = __ballot(in && k == prefix);
-        const int g0 = gt_before + __popcll(gts & below), e0 = eq_before + __popcll(eqs & below);
-        const int kept_before = g0 + (e0 < need_equal ? e0 : need_equal);
-        const bool stays = in && (k > prefix || (k == prefix && e0 < need_equal));
-        if (in && i < keep && !stays) holes[i - kept_before] = i;
-        if (stays && i >= keep) fills[keep - 1 - kept_before] = i;
-        if (stays && i < keep) {
-            if (copy_score) p.score_out[at] = score;
-            if (copy_pos) p.pos_out[at] = pos;
+    int gt_before = 0, eq_before = 0; // of the blocks before
+    for (int block = 0; block < blocks; ++block) {
+        if (blocks > 1) load(block);
+        int gt = 0, eq = 0;
+#pragma unroll
+        for (int k = 0; k < KEYS; ++k)
+            if (k < regs) {
+                gt += __popcll(__ballot(key[k] > prefix));
+                eq += __popcll(__ballot(key[k] == prefix));
+            }
+        __syncthreads();
+        if (lane == 0) {
+            seg_gt[wave] = gt;
+            seg_eq[wave] = eq;
         }
-        if (i == keep - 1) p.moves[blockIdx.x] = keep - kept_before - (stays ? 1 : 0);
-        gt_before += __popcll(gts);
-        eq_before += __popcll(eqs);
+        __syncthreads();
+        uint64_t in_place = 0; // bit k: this lane's token of register k stays where it is
+        int g_run = gt_before, e_run = eq_before;
+        for (int w = 0; w < WAVES; ++w) {
+            gt_before += seg_gt[w];
+            eq_before += seg_eq[w];
+            if (w < wave) {
+                g_run += seg_gt[w];
+                e_run += seg_eq[w];
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < KEYS; ++k)
+            if (k < regs) {
+                const int j = first_of(block, k), i = j + lane;
+                const uint64_t gts = __ballot(key[k] > prefix), eqs = __ballot(key[k] == prefix);
+                const int g0 = g_run + lanes_below(gts), e0 = e_run + lanes_below(eqs);
+                const int kept_before = g0 + (e0 < need_equal ? e0 : need_equal);
+                const bool stays = key[k] > prefix || (key[k] == prefix && e0 < need_equal); // (never past the end)
+                if (i < keep && !stays) holes[i - kept_before] = i;
+                if (stays && i >= keep) fills[keep - 1 - kept_before] = i;
+                if (i == keep - 1) p.moves[blockIdx.x] = keep - kept_before - (stays ? 1 : 0);
+                if (stays && i < keep) in_place |= uint64_t(1) << k;
+                g_run += __popcll(gts);
+                e_run += __popcll(eqs);
+            }
+        if (copy_score || copy_pos) {
+            for (int k0 = 0; k0 < KEYS; k0 += kBatch) {
+                float score[kBatch];
+                int32_t pos[kBatch];
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k)
+                    if ((in_place >> (k0 + k)) & 1) {
+                        const int64_t at = col.scores + uniform_token(p.pages, col.b, first_of(block, k0 + k)) + lane;
+                        score[k] = p.score_in[at];
+                        if (p.pos_in) pos[k] = p.pos_in[at];
+                    }
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k)
+                    if ((in_place >> (k0 + k)) & 1) {
+                        const int64_t at = col.scores + uniform_token(p.pages, col.b, first_of(block, k0 + k)) + lane;
+                        if (copy_score) p.score_out[at] = score[k];
+                        if (copy_pos) p.pos_out[at] = pos[k];
+                    }
+            }
+        }
     }
 }
 
 __global__ __launch_bounds__(256) void kv_evict_move_kernel(const EvictParams p) {
+    constexpr int kRows = 4; // rows whose piece a thread has in flight
     const int column = blockIdx.x / p.blocks_per_column;
     const int block = blockIdx.x - column * p.blocks_per_column;
-    const int count = p.moves[column];
     const EvictColumn col = evict_column(p, column);
     const int32_t* const holes = p.holes + (int64_t)column * p.max_moves;
     const int32_t* const fills = p.fills + (int64_t)column * p.max_moves;
     CacheAddr addr = p.addr;
     addr.layer += col.layer;
-    const int per_row = 2 * p.pieces;
-    const int64_t units = (int64_t)count * per_row;
-    for (int64_t u = (int64_t)block * 256 + threadIdx.x; u < units; u += (int64_t)p.blocks_per_column * 256) {
-        const int m = (int)(u / per_row);
-        const int r = (int)(u - (int64_t)m * per_row);
-        const int kv = r >= p.pieces, piece = r - kv * p.pieces;
-        const int64_t to = p.pages.token(col.b, holes[m]), from = p.pages.token(col.b, fills[m]);
-        const int64_t src = addr.row(from, kv, col.head) + 16 * piece, dst = addr.row(to, kv, col.head) + 16 * piece;
-        const uint4 q = *reinterpret_cast<const uint4*>(p.cache + src);
-        const uint32_t s = *reinterpret_cast<const uint32_t*>(p.scale + src / kQuantGroup);
-        *reinterpret_cast<uint4*>(p.cache + dst) = q;
-        *reinterpret_cast<uint32_t*>(p.scale + dst / kQuantGroup) = s;
+    // a thread keeps one piece of K or V and goes from row to row
+    const int per_row = 2 * p.pieces; // at most 32
+    const int rows_per_pass = 256 / per_row;
+    const int slot = threadIdx.x / per_row, r = threadIdx.x - slot * per_row;
+    if (slot >= rows_per_pass) return;
+    const int kv = r >= p.pieces, piece = r - kv * p.pieces;
+    const int count = p.moves[column], step = p.blocks_per_column * rows_per_pass;
+    const int64_t at0 = addr.row(0, kv, col.head) + 16 * piece;
+    for (int64_t m0 = (int64_t)block * rows_per_pass + slot; m0 < count; m0 += (int64_t)kRows * step) {
+        int64_t to[kRows], from[kRows];
+        uint4_vt q[kRows];
+        uint32_t s[kRows];
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            const int64_t m = m0 + (int64_t)i * step;
+            to[i] = from[i] = -1;
+            if (m < count) {
+                to[i] = p.pages.token(col.b, holes[m]);
+                from[i] = p.pages.token(col.b, fills[m]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            if (from[i] < 0) continue;
+            const int64_t src = at0 + from[i] * addr.stride_s;
+            q[i] = *reinterpret_cast<const uint4_vt*>(p.cache + src);
+            s[i] = *reinterpret_cast<const uint32_t*>(p.scale + src / kQuantGroup);
+        }
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            if (from[i] < 0) continue;
+            const int64_t dst = at0 + to[i] * addr.stride_s;
+            *reinterpret_cast<uint4_vt*>(p.cache + dst) = q[i];
+            *reinterpret_cast<uint32_t*>(p.scale + dst / kQuantGroup) = s[i];
+        }
         if (r == 0) {
-            p.score_out[col.scores + to] = p.score_in[col.scores + from];
-            if (p.pos_in) p.pos_out[col.scores + to] = p.pos_in[col.scores + from];
+#pragma unroll
+            for (int i = 0; i < kRows; ++i) {
+                if (from[i] < 0) continue;
+                p.score_out[col.scores + to[i]] = p.score_in[col.scores + from[i]];
+                if (p.pos_in) p.pos_out[col.scores + to[i]] = p.pos_in[col.scores + from[i]];
+            }
         }
     }
 }
@@ -234,12 +320,20 @@ pplhip_retcode launch_kv_evict(const pplhip_kv_evict_args* a, int64_t max_moves,
     p.moves = (int32_t*)ws;
     p.holes = p.moves + columns;
     p.fills = p.holes + columns * max_moves;
-    hipLaunchKernelGGL(kv_evict_choose_kernel, dim3((unsigned)columns), dim3(kChooseThreads), 0, stream, p);
+    // (a column's keys fit the registers of the smallest workgroup that holds them: many short columns run side by side)
+    const dim3 cols((unsigned)columns);
+    if (a->max_kvlen <= 256 * 16)
+        hipLaunchKernelGGL((kv_evict_choose_kernel<256, 16>), cols, dim3(256), 0, stream, p);
+    else if (a->max_kvlen <= 1024 * 16)
+        hipLaunchKernelGGL((kv_evict_choose_kernel<1024, 16>), cols, dim3(1024), 0, stream, p);
+    else
+        hipLaunchKernelGGL((kv_evict_choose_kernel<1024, 64>), cols, dim3(1024), 0, stream, p);
     PPLHIP_CHECK_LAUNCH("kv_evict choose");
     // how many rows move is known on the device only: enough workgroups to fill the chip a few times over, each of which
     // walks its share of the column's list
-    const int64_t most = (max_moves * 2 * p.pieces + 255) / 256;
-    int64_t per_column = (8192 + columns - 1) / columns;
+    const int64_t rows_per_pass = 256 / (2 * p.pieces);
+    const int64_t most = (max_moves + rows_per_pass - 1) / rows_per_pass;
+    int64_t per_column = (2048 + columns - 1) / columns;
     if (per_column > most) per_column = most;
     if (per_column < 1) per_column = 1;
     p.blocks_per_column = (int32_t)per_column;
@@ -290,7 +384,7 @@ __global__ __launch_bounds__(256) void kv_accept_kernel(const AcceptParams p) {
     int64_t prev = -1;
     for (int64_t i0 = 0; i0 < n; i0 += kRows) {
         int64_t from[kRows];
-        uint4 q[kRows];
+        uint4_vt q[kRows];
         uint32_t s[kRows];
 #pragma unroll
         for (int i = 0; i < kRows; ++i) from[i] = i0 + i < n ? path[i0 + i] : -1;
@@ -306,7 +400,7 @@ __global__ __launch_bounds__(256) void kv_accept_kernel(const AcceptParams p) {
         for (int i = 0; i < kRows; ++i) {
             if (i < rows && from[i] != i0 + i) {
                 const int64_t row = addr.row(p.pages.token(b, start + from[i]), kv, head) + 16 * piece;
-                q[i] = *reinterpret_cast<const uint4*>(p.cache + row);
+                q[i] = *reinterpret_cast<const uint4_vt*>(p.cache + row);
                 s[i] = *reinterpret_cast<const uint32_t*>(p.scale + row / kQuantGroup);
             }
         }
@@ -314,7 +408,7 @@ __global__ __launch_bounds__(256) void kv_accept_kernel(const AcceptParams p) {
         for (int i = 0; i < kRows; ++i) {
             if (i < rows && from[i] != i0 + i) {
                 const int64_t row = addr.row(p.pages.token(b, start + i0 + i), kv, head) + 16 * piece;
-                *reinterpret_cast<uint4*>(p.cache + row) = q[i];
+                *reinterpret_cast<uint4_vt*>(p.cache + row) = q[i];
                 *reinterpret_cast<uint32_t*>(p.scale + row / kQuantGroup) = s[i];
             }
         }

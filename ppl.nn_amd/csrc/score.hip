@@ -140,8 +140,7 @@ __global__ __launch_bounds__(256, 2) void kv_score_kernel(const ScoreParams p) {
     const float mine = g == 0 ? w[0] : g == 1 ? w[1] : g == 2 ? w[2] : w[3];
     const int64_t j = key0 + lane;
     if (j < kvlen) {
-        const PageMap pages{p.view.cachestarts, p.view.cs_stride_b, p.view.page_shift};
-        const int64_t at = p.score_offset + kvh * p.score_stride_h + pages.token(b, j);
+        const int64_t at = p.score_offset + kvh * p.score_stride_h + uniform_token(p.view.pages, b, (int)key0) + lane;
         p.score_out[at] = (j < start ? p.score_in[at] : 0.f) + mine;
         if (p.position && j >= start) p.position[at] = (int32_t)p.position_idx[s0 + (j - start)];
     }
@@ -154,9 +153,10 @@ pplhip_retcode launch_kv_score(const pplhip_kv_score_args* a, hipStream_t stream
     p.position_idx = a->d_position_idx;
     p.seqstarts = a->d_seqstarts;
     p.kvstarts = a->d_kvstarts;
-    p.view = CacheView{(const int8_t*)a->d_cache, (const half_t*)a->d_scale, a->d_cachestarts, a->cachestart_stride_b,
+    p.view = CacheView{(const int8_t*)a->d_cache, (const half_t*)a->d_scale,
+                       PageMap{a->d_cachestarts, a->cachestart_stride_b, page_shift_of(a->cache_mode, a->page_size)},
                        CacheAddr{a->cache_stride_s, a->cache_stride_l, a->cache_stride_h, a->cache_stride_kv, a->layer_idx},
-                       page_shift_of(a->cache_mode, a->page_size), a->head_dim};
+                       a->head_dim};
     p.score_in = a->d_score_in;
     p.score_out = a->d_score_out;
     p.position = a->d_position;

@@ -777,9 +777,10 @@ pplhip_retcode launch_tree_attention(const pplhip_tree_attention_args* a, int64_
     p.mask = a->d_tree_mask;
     p.seqstarts = a->d_seqstarts;
     p.kvstarts = a->d_kvstarts;
-    p.view = CacheView{(const int8_t*)a->d_cache, (const half_t*)a->d_scale, a->d_cachestarts, a->cachestart_stride_b,
+    p.view = CacheView{(const int8_t*)a->d_cache, (const half_t*)a->d_scale,
+                       PageMap{a->d_cachestarts, a->cachestart_stride_b, page_shift_of(a->cache_mode, a->page_size)},
                        CacheAddr{a->cache_stride_s, a->cache_stride_l, a->cache_stride_h, a->cache_stride_kv, a->layer_idx},
-                       page_shift_of(a->cache_mode, a->page_size), a->head_dim};
+                       a->head_dim};
     p.out = (half_t*)a->d_output;
     p.lse = (float*)a->d_lse;
     p.batch = (int32_t)a->batch;
