@@ -3,8 +3,8 @@
 //
 // With the rows' log-sums known the weights need no second look at the keys: one pass over K (the V half of the slab is
 // not touched), every key's sum in one place. A wave owns 64 keys: it holds them as matrix-core operands for the whole
-// kernel (each cached byte is read and dequantised once, whatever the number of rows) and streams the rows past them,
-// 16 at a time: S = Q K^T with v_mfma_f32_16x16x32_f16, a key living in the 16 lanes' same column, so a key's sum runs
+// kernel (each cached byte is read and dequantised once, whatever the number of rows) and the rows pass by, 16 at a time
+// out of LDS, where the four waves share them: S = Q K^T with v_mfma_f32_16x16x32_f16, a key living in the 16 lanes' same column, so a key's sum runs
 // in one register per lane over all rows and is joined over the four lane groups once at the end. No atomics: the order
 // of the sum is fixed.
 #include "cache_tile.h"
@@ -29,13 +29,14 @@ struct ScoreParams {
 
 constexpr int kScoreWaveKeys = 64;
 constexpr int kScoreKeys = 4 * kScoreWaveKeys; // keys per workgroup
-constexpr int kScoreRows = 256; // rows whose log-sums are held in LDS at a time
+constexpr int kScoreRows = 128; // rows held in LDS at a time: they take the place of the key tiles
 
 template <int DH>
 __global__ __launch_bounds__(256, 2) void kv_score_kernel(const ScoreParams p) {
     constexpr int LDR = kKeyRow<DH>;
     constexpr int KC2 = DH / 32;
-    __shared__ __attribute__((aligned(16))) half_t lds[4 * kTileKeys * LDR];
+    __shared__ __attribute__((aligned(16))) half_t lds[4 * kTileKeys * LDR]; // key tiles, then rows of queries
+    static_assert(kScoreRows <= 4 * kTileKeys, "the rows fit the tiles' place");
     __shared__ __attribute__((aligned(16))) float row_lse[kScoreRows]; // in units of log2
     __shared__ __attribute__((aligned(16))) int row_last[kScoreRows]; // last key of the workgroup's block the row sees, or -1
 
@@ -46,14 +47,13 @@ __global__ __launch_bounds__(256, 2) void kv_score_kernel(const ScoreParams p) {
     const int kvh = blockIdx.x % p.kv_heads;
     const int rest = blockIdx.x / p.kv_heads;
     const int b = rest / p.key_blocks;
-    const int64_t block0 = (int64_t)(rest - b * p.key_blocks) * kScoreKeys;
+    const int block0 = (rest - b * p.key_blocks) * kScoreKeys;
     const const_tab64_t seqstarts = (const_tab64_t)p.seqstarts, kvstarts = (const_tab64_t)p.kvstarts;
-    const int64_t s0 = seqstarts[b], L = seqstarts[b + 1] - s0;
-    const int64_t kvlen = kvstarts[b + 1] - kvstarts[b];
+    const int64_t s0 = seqstarts[b];
+    const int L = (int)(seqstarts[b + 1] - s0), kvlen = (int)(kvstarts[b + 1] - kvstarts[b]);
     if (L <= 0 || block0 >= kvlen) return;
-    const int64_t start = kvlen - L;
-    const int64_t rows = L * p.rep;
-    const int64_t key0 = block0 + wave * kScoreWaveKeys;
+    const int start = kvlen - L, rows = L * p.rep;
+    const int key0 = block0 + wave * kScoreWaveKeys;
     half_t* const tile = lds + wave * kTileKeys * LDR;
 
     // ---- the wave's keys as B operands: key 16 * kb + r_lane, positions 32 * kc + 8 * g .. + 7 of its LDS row
@@ -63,8 +63,8 @@ __global__ __launch_bounds__(256, 2) void kv_score_kernel(const ScoreParams p) {
         CacheTile<DH> raw[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int kv0 = (int)(key0 + h * kTileKeys < kvlen ? key0 + h * kTileKeys : key0);
-            raw[h].fetch(p.view, p.view.key_row(b, kv0, kvh), kv0, (int)kvlen);
+            const int kv0 = key0 + h * kTileKeys < kvlen ? key0 + h * kTileKeys : key0;
+            raw[h].fetch(p.view, p.view.key_row(b, kv0, kvh), kv0, kvlen);
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -79,18 +79,26 @@ __global__ __launch_bounds__(256, 2) void kv_score_kernel(const ScoreParams p) {
         }
     }
     float w[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int64_t chunk = 0; chunk < rows; chunk += kScoreRows) {
-        const int n = rows - chunk < kScoreRows ? (int)(rows - chunk) : kScoreRows;
-        if (chunk) __syncthreads();
-        {
+    for (int chunk = 0; chunk < rows; chunk += kScoreRows) {
+        const int n = rows - chunk < kScoreRows ? rows - chunk : kScoreRows;
+        __syncthreads(); // (the key tiles, or the rows before, have been read)
+        // rows of the chunk, 16 bytes (one group) a thread at a time
+        const int groups = hd / 8;
+#pragma unroll 2
+        for (int x = threadIdx.x; x < n * groups; x += 256) {
+            const int r = x / groups, group = x - r * groups;
+            const int row = chunk + r, t = row / p.rep;
+            const half_t* src = p.q + ((s0 + t) * p.num_heads + kvh * p.rep + (row - t * p.rep)) * hd + 8 * group;
+            *reinterpret_cast<half8_t*>(lds + r * LDR + 8 * group) = *reinterpret_cast<const half8_t*>(src);
+        }
+        if (threadIdx.x < kScoreRows) {
             float l = 0.f;
             int last = -1;
             if ((int)threadIdx.x < n) {
-                const int64_t row = chunk + threadIdx.x;
-                const int64_t t = row / p.rep;
+                const int row = chunk + threadIdx.x, t = row / p.rep;
                 l = p.lse[(s0 + t) * p.num_heads + kvh * p.rep + (row - t * p.rep)] * 1.44269504088896f;
-                const int64_t lim = start + t - block0;
-                if (l != -INFINITY) last = lim < -1 ? -1 : lim > kScoreKeys ? kScoreKeys : (int)lim;
+                const int lim = start + t - block0;
+                if (l != -INFINITY) last = lim < -1 ? -1 : lim;
             }
             row_lse[threadIdx.x] = l;
             row_last[threadIdx.x] = last;
@@ -98,33 +106,42 @@ __global__ __launch_bounds__(256, 2) void kv_score_kernel(const ScoreParams p) {
         __syncthreads();
         if (!have_keys) continue;
         for (int r0 = 0; r0 < n; r0 += 16) {
-            const int64_t row = chunk + r0 + r_lane < rows ? chunk + r0 + r_lane : rows - 1;
-            const int64_t t = row / p.rep;
-            const half_t* qp = p.q + ((s0 + t) * p.num_heads + kvh * p.rep + (row - t * p.rep)) * hd;
+            const int r = r0 + r_lane < n ? r0 + r_lane : n - 1;
             half8_t qf[KC2];
 #pragma unroll
             for (int kc = 0; kc < KC2; ++kc) {
                 const int channel = channel_at<DH>(32 * kc + 8 * g);
-                if (channel < hd) {
-                    qf[kc] = *reinterpret_cast<const half8_t*>(qp + channel);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) qf[kc][e] = (half_t)0.f;
-                }
+                qf[kc] = *reinterpret_cast<const half8_t*>(lds + r * LDR + (channel < hd ? channel : 0));
+                if (hd < DH && channel >= hd) qf[kc] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
             }
             const float4_t lse = *reinterpret_cast<const float4_t*>(&row_lse[r0 + 4 * g]);
             const int4 last = *reinterpret_cast<const int4*>(&row_last[r0 + 4 * g]);
             const int lim[4] = {last.x, last.y, last.z, last.w};
+            // every row sees every key of the wave (and has a distribution): nothing to hide
+            const int least = min(min(lim[0], lim[1]), min(lim[2], lim[3]));
+            const bool all = __all(least >= (wave + 1) * kScoreWaveKeys - 1);
+            float4_t acc[4];
+#pragma unroll
+            for (int kb = 0; kb < 4; ++kb) acc[kb] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int kc = 0; kc < KC2; ++kc)
+#pragma unroll
+                for (int kb = 0; kb < 4; ++kb)
+                    acc[kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qf[kc], kf[kb][kc], acc[kb], 0, 0, 0);
+            if (all) {
+#pragma unroll
+                for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        w[kb] += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[kb][e], p.scale_log2, -lse[e]));
+                continue;
+            }
 #pragma unroll
             for (int kb = 0; kb < 4; ++kb) {
-                float4_t acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int kc = 0; kc < KC2; ++kc)
-                    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(qf[kc], kf[kb][kc], acc, 0, 0, 0);
                 const int key = wave * kScoreWaveKeys + 16 * kb + r_lane; // within the workgroup's block
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[e], p.scale_log2, -lse[e]));
+                    const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[kb][e], p.scale_log2, -lse[e]));
                     w[kb] += key <= lim[e] ? pr : 0.f;
                 }
             }
@@ -138,9 +155,9 @@ __global__ __launch_bounds__(256, 2) void kv_score_kernel(const ScoreParams p) {
     }
     // lane group g writes key block g: 64 consecutive keys, one per lane
     const float mine = g == 0 ? w[0] : g == 1 ? w[1] : g == 2 ? w[2] : w[3];
-    const int64_t j = key0 + lane;
+    const int j = key0 + lane;
     if (j < kvlen) {
-        const int64_t at = p.score_offset + kvh * p.score_stride_h + uniform_token(p.view.pages, b, (int)key0) + lane;
+        const int64_t at = p.score_offset + kvh * p.score_stride_h + uniform_token(p.view.pages, b, key0) + lane;
         p.score_out[at] = (j < start ? p.score_in[at] : 0.f) + mine;
         if (p.position && j >= start) p.position[at] = (int32_t)p.position_idx[s0 + (j - start)];
     }
