@@ -197,6 +197,16 @@ struct SharedTile {
     // finite_values: V pieces that may not be finite become zeros; returns the rows of those this thread had
     __device__ inline uint32_t stash(half_t* k_tile, half_t* v_tile, int head_dim, bool finite_values) const {
         uint32_t odd = 0;
+        if (!finite_values && head_dim == DH) { // (nearly every tile)
+#pragma unroll
+            for (int n = 0; n < NLD; ++n) {
+                int kv, row, piece;
+                place(n, &kv, &row, &piece);
+                if (row >= kTileKeys) break;
+                stash_piece<DH>(kv ? v_tile + row * kValueRow<DH> : k_tile + row * kKeyRow<DH>, piece, q[n], s[n]);
+            }
+            return 0;
+        }
 #pragma unroll
         for (int n = 0; n < NLD; ++n) {
             int kv, row, piece;

@@ -72,7 +72,7 @@ __global__ __launch_bounds__(T) void kv_evict_choose_kernel(const EvictParams p)
     // copies of the digit counts: scores share their leading bits, so lanes would queue at one counter; few keys do not
     // pay for clearing and adding up many
     constexpr int kHistCopies = T * KEYS > 4096 ? 16 : 4;
-    constexpr int kBatch = KEYS < 16 ? KEYS : 16; // tokens whose loads a thread has in flight
+    constexpr int kBatch = 8; // tokens whose loads a thread has in flight
     __shared__ uint32_t hist[256 * kHistCopies];
     __shared__ uint32_t wave_sum[4];
     __shared__ uint32_t found[2]; // digit, rows above it
@@ -233,7 +233,6 @@ __global__ __launch_bounds__(T) void kv_evict_choose_kernel(const EvictParams p)
 }
 
 __global__ __launch_bounds__(256) void kv_evict_move_kernel(const EvictParams p) {
-    constexpr int kRows = 4; // rows whose piece a thread has in flight
     const int column = blockIdx.x / p.blocks_per_column;
     const int block = blockIdx.x - column * p.blocks_per_column;
     const EvictColumn col = evict_column(p, column);
@@ -249,40 +248,16 @@ __global__ __launch_bounds__(256) void kv_evict_move_kernel(const EvictParams p)
     const int kv = r >= p.pieces, piece = r - kv * p.pieces;
     const int count = p.moves[column], step = p.blocks_per_column * rows_per_pass;
     const int64_t at0 = addr.row(0, kv, col.head) + 16 * piece;
-    for (int64_t m0 = (int64_t)block * rows_per_pass + slot; m0 < count; m0 += (int64_t)kRows * step) {
-        int64_t to[kRows], from[kRows];
-        uint4_vt q[kRows];
-        uint32_t s[kRows];
-#pragma unroll
-        for (int i = 0; i < kRows; ++i) {
-            const int64_t m = m0 + (int64_t)i * step;
-            to[i] = from[i] = -1;
-            if (m < count) {
-                to[i] = p.pages.token(col.b, holes[m]);
-                from[i] = p.pages.token(col.b, fills[m]);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < kRows; ++i) {
-            if (from[i] < 0) continue;
-            const int64_t src = at0 + from[i] * addr.stride_s;
-            q[i] = *reinterpret_cast<const uint4_vt*>(p.cache + src);
-            s[i] = *reinterpret_cast<const uint32_t*>(p.scale + src / kQuantGroup);
-        }
-#pragma unroll
-        for (int i = 0; i < kRows; ++i) {
-            if (from[i] < 0) continue;
-            const int64_t dst = at0 + to[i] * addr.stride_s;
-            *reinterpret_cast<uint4_vt*>(p.cache + dst) = q[i];
-            *reinterpret_cast<uint32_t*>(p.scale + dst / kQuantGroup) = s[i];
-        }
+    for (int64_t m = (int64_t)block * rows_per_pass + slot; m < count; m += step) {
+        const int64_t to = p.pages.token(col.b, holes[m]), from = p.pages.token(col.b, fills[m]);
+        const int64_t src = at0 + from * addr.stride_s, dst = at0 + to * addr.stride_s;
+        const uint4_vt q = *reinterpret_cast<const uint4_vt*>(p.cache + src);
+        const uint32_t s = *reinterpret_cast<const uint32_t*>(p.scale + src / kQuantGroup);
+        __builtin_nontemporal_store(q, reinterpret_cast<uint4_vt*>(p.cache + dst)); // (not read again by this call)
+        *reinterpret_cast<uint32_t*>(p.scale + dst / kQuantGroup) = s;
         if (r == 0) {
-#pragma unroll
-            for (int i = 0; i < kRows; ++i) {
-                if (from[i] < 0) continue;
-                p.score_out[col.scores + to[i]] = p.score_in[col.scores + from[i]];
-                if (p.pos_in) p.pos_out[col.scores + to[i]] = p.pos_in[col.scores + from[i]];
-            }
+            p.score_out[col.scores + to] = p.score_in[col.scores + from];
+            if (p.pos_in) p.pos_out[col.scores + to] = p.pos_in[col.scores + from];
         }
     }
 }
@@ -333,7 +308,7 @@ pplhip_retcode launch_kv_evict(const pplhip_kv_evict_args* a, int64_t max_moves,
     // walks its share of the column's list
     const int64_t rows_per_pass = 256 / (2 * p.pieces);
     const int64_t most = (max_moves + rows_per_pass - 1) / rows_per_pass;
-    int64_t per_column = (2048 + columns - 1) / columns;
+    int64_t per_column = (8192 + columns - 1) / columns;
     if (per_column > most) per_column = most;
     if (per_column < 1) per_column = 1;
     p.blocks_per_column = (int32_t)per_column;

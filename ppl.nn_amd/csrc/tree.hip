@@ -45,7 +45,7 @@ struct TreeParams {
 
 constexpr int kTreeWaves = 4; // of tree_keys_kernel
 constexpr int64_t kPieceCost = 4; // what starting and finishing a row tile costs, in key tiles
-constexpr int64_t kMinRangeTiles = 8; // a range is at least this long: two key tiles per wave
+constexpr int64_t kMinRangeTiles = 16; // a range is at least this long: four key tiles per wave of the smallest kernel
 // The reference point m of a row's exponents need not be its running maximum: it only moves when a score passes it by
 // more than 2^kSlack, so that most tiles need neither a maximum across lanes nor a rescaling. Weights are held as
 // exp2(x - m + kProbShift), at most 2^15 in fp16 (the operand of the second product); a weight keeps fp16's full
@@ -200,19 +200,17 @@ struct RowState {
     // scores of the rows against those keys: s[n][tb][e] belongs to key 16 * tb + 4 * g + e
     __device__ inline void scores(const KeyOperands& kf, float (&s)[N][2][4]) const {
 #pragma unroll
-        for (int tb = 0; tb < 2; ++tb) {
-            float4_t acc[N];
-#pragma unroll
-            for (int n = 0; n < N; ++n) acc[n] = float4_t{0.f, 0.f, 0.f, 0.f};
+        for (int n = 0; n < N; ++n) {
+            float4_t acc[2] = {float4_t{0.f, 0.f, 0.f, 0.f}, float4_t{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
             for (int kc = 0; kc < DH / 32; ++kc)
 #pragma unroll
-                for (int n = 0; n < N; ++n)
-                    acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[tb][kc], qf[n][kc], acc[n], 0, 0, 0);
+                for (int tb = 0; tb < 2; ++tb)
+                    acc[tb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[tb][kc], qf[n][kc], acc[tb], 0, 0, 0);
 #pragma unroll
-            for (int n = 0; n < N; ++n)
+            for (int tb = 0; tb < 2; ++tb)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[n][tb][e] = acc[n][e];
+                for (int e = 0; e < 4; ++e) s[n][tb][e] = acc[tb][e];
         }
     }
 
@@ -295,9 +293,10 @@ struct RowState {
     // o += weights x those rows
     __device__ inline void values(const ValueOperands& vf, const half8_t (&pp)[N]) {
 #pragma unroll
-        for (int i = 0; i < DH / 16; ++i)
+        for (int n = 0; n < N; ++n) {
 #pragma unroll
-            for (int n = 0; n < N; ++n) o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[i], pp[n], o[n][i], 0, 0, 0);
+            for (int i = 0; i < DH / 16; ++i) o[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[i], pp[n], o[n][i], 0, 0, 0);
+        }
     }
 
     // Value pieces that may not be finite are zeros in the tiles (a key can be hidden from a row: its weight there is 0,
@@ -692,34 +691,56 @@ __global__ __launch_bounds__(W * 64, tree_waves_per_simd(DH, NB)) void tree_rows
 // tile's partials: the last piece of the range before it, then the first pieces of the ranges behind it.
 template <int DH>
 __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeParams p, const int ROWS) {
+    constexpr int kParts = 4; // partials a thread has in flight
     const int range = 1 + blockIdx.x / p.kv_heads;
     const int kvh = blockIdx.x % p.kv_heads;
     const const_tab64_t st = (const_tab64_t)p.range_start;
     const int64_t b = st[3 * range], row_tile = st[3 * range + 1];
     if (b < 0 || st[3 * range + 2] == 0) return; // starts nothing, or starts with its row tile
     if (st[3 * (range - 1)] == b && st[3 * (range - 1) + 1] == row_tile && st[3 * (range - 1) + 2] != 0) return;
+    // how far the row tile's ranges go: 64 of them looked at a time
     int last = range;
-    while (last + 1 < p.num_ranges && st[3 * (last + 1)] == b && st[3 * (last + 1) + 1] == row_tile &&
-           st[3 * (last + 1) + 2] != 0)
-        ++last;
+    for (int first = range;; first += 64) {
+        const int k = first + (int)(threadIdx.x & 63);
+        const int64_t* const e = p.range_start + 3 * (int64_t)(k < p.num_ranges ? k : range);
+        const uint64_t other = __ballot(k >= p.num_ranges || e[0] != b || e[1] != row_tile || e[2] == 0);
+        last = first + (other ? __builtin_ctzll(other) : 64) - 1;
+        if (other) break;
+    }
     const int64_t s0 = p.seqstarts[b], rows = (p.seqstarts[b + 1] - s0) * p.rep;
     const int64_t base = (int64_t)kvh * 2 * p.num_ranges;
     for (int x = blockIdx.y * 256 + threadIdx.x; x < ROWS * (DH / 4); x += 256 * gridDim.y) {
         const int r = x / (DH / 4), d = (x - r * (DH / 4)) * 4;
         const int row = (int)row_tile * ROWS + r;
         if (row >= rows) continue;
+        const int parts = last - range + 2;
+        auto slot = [&](int k) { return (base + (k == 0 ? 2 * range - 1 : 2 * (range - 1 + k))) * ROWS + r; };
         float m = -INFINITY, l = 0.f;
         float4_t a = {0.f, 0.f, 0.f, 0.f};
-        for (int k = range - 1; k <= last; ++k) {
-            const int64_t at = (base + (k < range ? 2 * k + 1 : 2 * k)) * ROWS + r;
-            const float2 ml = p.part_ml[at];
-            const float4_t v = *reinterpret_cast<const float4_t*>(p.part_o + at * DH + d);
-            const float m_new = fmaxf(m, ml.x);
+        for (int k0 = 0; k0 < parts; k0 += kParts) {
+            float2 ml[kParts];
+            float4_t v[kParts];
+#pragma unroll
+            for (int k = 0; k < kParts; ++k) { // (past the last part: the first again, with no weight)
+                const int64_t at = slot(k0 + k < parts ? k0 + k : 0);
+                ml[k] = p.part_ml[at];
+                v[k] = *reinterpret_cast<const float4_t*>(p.part_o + at * DH + d);
+            }
+            float m_new = m;
+#pragma unroll
+            for (int k = 0; k < kParts; ++k) m_new = fmaxf(m_new, ml[k].x);
             const float m_safe = m_new == -INFINITY ? 0.f : m_new;
-            const float fo = __builtin_amdgcn_exp2f(m - m_safe), fn = __builtin_amdgcn_exp2f(ml.x - m_safe);
-            l = l * fo + ml.y * fn;
-            a = a * fo + v * fn;
+            const float f0 = __builtin_amdgcn_exp2f(m - m_safe);
+            l *= f0;
+            a *= f0;
             m = m_new;
+#pragma unroll
+            for (int k = 0; k < kParts; ++k) {
+                if (k0 + k >= parts) continue;
+                const float f = __builtin_amdgcn_exp2f(ml[k].x - m_safe);
+                l += ml[k].y * f;
+                a += v[k] * f;
+            }
         }
         finish_row(p, s0, row, kvh, channel_at<DH>(d), a, m, l);
     }
