@@ -49,11 +49,23 @@ struct CacheView {
     PageMap pages;
     CacheAddr addr;
     int32_t head_dim;
+};
 
-    // element offset of the K row of key j of sequence b (both wave-uniform; a run of 32 keys from a multiple of 32
-    // lies in one page: pages are powers of two of at least 64 tokens)
-    __device__ inline int64_t key_row(int b, int j, int kvh) const {
-        return addr.row(uniform_token(pages, b, j), 0, kvh);
+// One sequence's rows of one kv head, with what does not change along it worked out once.
+struct SequenceRows {
+    const_tab64_t pages; // the sequence's page-table row (paged)
+    int64_t head_row; // paged: element offset of slab token 0's K row; contiguous: of the sequence's key 0
+    int32_t stride_s, page_shift;
+
+    __device__ inline SequenceRows(const CacheView& v, int b, int kvh)
+        : pages((const_tab64_t)v.pages.cachestarts + b * v.pages.stride_b), head_row(v.addr.row(0, 0, kvh)),
+          stride_s((int32_t)v.addr.stride_s), page_shift(v.pages.page_shift) {
+        if (page_shift == 0) head_row = v.addr.row(((const_tab64_t)v.pages.cachestarts)[b], 0, kvh);
+    }
+    // element offset of the K row of key j (wave-uniform; a run of 32 keys from a multiple of 32 lies in one page)
+    __device__ inline int64_t key_row(int j) const {
+        if (page_shift == 0) return head_row + (int64_t)j * stride_s;
+        return head_row + (pages[j >> page_shift] + (j & ((1 << page_shift) - 1))) * (int64_t)stride_s;
     }
 };
 
@@ -164,9 +176,10 @@ struct CacheTile {
     }
 };
 
-// The same for a workgroup of W waves that shares the tile: a thread's pieces of the tile's K and V rows.
-template <int DH, int W>
+// The same for four waves that bring a tile together: a thread's pieces of the tile's K and V rows.
+template <int DH>
 struct SharedTile {
+    static constexpr int W = 4;
     static constexpr int PIECES = DH / 16;
     static constexpr int ALL = 2 * kTileKeys * PIECES; // K's, then V's
     static constexpr int NLD = (ALL + 64 * W - 1) / (64 * W);
@@ -175,7 +188,7 @@ struct SharedTile {
 
     // Piece n of this thread: K or V (the same for the whole wave: a tile's K pieces are a multiple of 64), row, piece of it
     __device__ static inline void place(int n, int* kv, int* row, int* piece) {
-        const int first = 64 * (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) + W * n); // the wave's first piece
+        const int first = 64 * ((__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & (W - 1)) + W * n); // the wave's first piece
         *kv = first >= kTileKeys * PIECES;
         const uint32_t c = (threadIdx.x & 63) + first - (*kv ? kTileKeys * PIECES : 0);
         *row = c / PIECES;

@@ -60,11 +60,12 @@ __global__ __launch_bounds__(256, 2) void kv_score_kernel(const ScoreParams p) {
     half8_t kf[4][KC2];
     const bool have_keys = key0 < kvlen;
     if (have_keys) {
+        const SequenceRows seq(p.view, b, kvh);
         CacheTile<DH> raw[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int kv0 = key0 + h * kTileKeys < kvlen ? key0 + h * kTileKeys : key0;
-            raw[h].fetch(p.view, p.view.key_row(b, kv0, kvh), kv0, kvlen);
+            raw[h].fetch(p.view, seq.key_row(kv0), kv0, kvlen);
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {

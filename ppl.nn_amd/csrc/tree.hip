@@ -231,29 +231,34 @@ struct RowState {
         }
     }
 
-    // moves a row's reference point where a score passes it by too much
-    __device__ inline void settle(float scale_log2, const float (&s)[N][2][4]) {
-        float top[N];
-        bool moves = false;
+    // largest of the lane's scores of every row
+    __device__ static inline void largest(const float (&s)[N][2][4], float (&top)[N]) {
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
+        for (int n = 0; n < N; ++n)
             top[n] = fmaxf(fmaxf(fmaxf(s[n][0][0], s[n][0][1]), fmaxf(s[n][0][2], s[n][0][3])),
                            fmaxf(fmaxf(s[n][1][0], s[n][1][1]), fmaxf(s[n][1][2], s[n][1][3])));
+    }
+    // whether one of them passes its row's reference point by too much
+    __device__ inline bool passes(float scale_log2, const float (&top)[N]) const {
+        bool moves = false;
+#pragma unroll
+        for (int n = 0; n < N; ++n)
             moves |= (__builtin_fmaf(top[n], scale_log2, shift[n]) > kProbShift + kSlack) |
                      ((m[n] == -INFINITY) & (top[n] > -INFINITY));
-        }
-        if (__any(moves)) { // (rows without a key so far keep m = -inf: weights exp2(-inf) = 0)
+        return __any(moves);
+    }
+    // moves the reference points there (rows without a key so far keep m = -inf: weights exp2(-inf) = 0)
+    __device__ inline void settle(float scale_log2, const float (&top)[N]) {
 #pragma unroll
-            for (int n = 0; n < N; ++n) {
-                const float m_new = fmaxf(m[n], max_over_groups(top[n]));
-                const float ref = m_new == -INFINITY ? 0.f : m_new;
-                const float alpha = __builtin_amdgcn_exp2f((m[n] - ref) * scale_log2);
-                m[n] = m_new;
-                shift[n] = kProbShift - ref * scale_log2;
-                l[n] *= alpha;
+        for (int n = 0; n < N; ++n) {
+            const float m_new = fmaxf(m[n], max_over_groups(top[n]));
+            const float ref = m_new == -INFINITY ? 0.f : m_new;
+            const float alpha = __builtin_amdgcn_exp2f((m[n] - ref) * scale_log2);
+            m[n] = m_new;
+            shift[n] = kProbShift - ref * scale_log2;
+            l[n] *= alpha;
 #pragma unroll
-                for (int i = 0; i < DH / 16; ++i) o[n][i] *= alpha;
-            }
+            for (int i = 0; i < DH / 16; ++i) o[n][i] *= alpha;
         }
     }
 
@@ -352,7 +357,7 @@ struct TreePiece {
     int32_t start, kvlen, rows, row0; // row0: first row of the tile
     int32_t key_tile, stop_tile; // key tiles to look at (causal rows see nothing past their own token)
     bool whole; // all the row tile's keys are in this piece
-    int64_t slot; // else: where its partial goes
+    int32_t slot; // else: where its partial goes
 };
 
 // Calls `piece` for every piece of workgroup (range, kvh)'s range.
@@ -364,7 +369,8 @@ __device__ inline void walk_range(const TreeParams& p, int range, int kvh, F&& p
     int64_t left = uniform64(rs.length);
     int b = __builtin_amdgcn_readfirstlane(rs.b), row_tile = __builtin_amdgcn_readfirstlane(rs.row_tile),
         key_tile = __builtin_amdgcn_readfirstlane(rs.key_tile);
-    int first_b = -1, first_row_tile = 0, first_key_tile = 0;
+    bool first = true;
+    if (kvh == 0 && threadIdx.x == 0) p.range_start[3 * range] = -1; // (until a piece is found)
     while (left > 0 && b < p.batch) {
         TreePiece t;
         t.b = b;
@@ -381,11 +387,12 @@ __device__ inline void walk_range(const TreeParams& p, int range, int kvh, F&& p
         }
         const int end_tile = key_tile + left < key_tiles ? key_tile + (int)left : key_tiles;
         if (key_tile < end_tile) {
-            if (first_b < 0) {
-                first_b = b;
-                first_row_tile = row_tile;
-                first_key_tile = key_tile;
+            if (first && kvh == 0 && threadIdx.x == 0) {
+                p.range_start[3 * range] = b;
+                p.range_start[3 * range + 1] = row_tile;
+                p.range_start[3 * range + 2] = key_tile;
             }
+            first = false;
             t.start = t.kvlen - L;
             t.row0 = row_tile * ROWS;
             t.key_tile = key_tile;
@@ -396,17 +403,12 @@ __device__ inline void walk_range(const TreeParams& p, int range, int kvh, F&& p
                 t.stop_tile = last < end_tile ? last : end_tile;
             }
             t.whole = key_tile == 0 && end_tile == key_tiles;
-            t.slot = (int64_t)kvh * 2 * p.num_ranges + 2 * (int64_t)range + (key_tile == 0 ? 1 : 0);
+            t.slot = 2 * (kvh * p.num_ranges + range) + (key_tile == 0 ? 1 : 0);
             piece(t);
         }
         left -= key_tiles + kPieceCost - key_tile;
         ++row_tile;
         key_tile = 0;
-    }
-    if (kvh == 0 && threadIdx.x == 0) {
-        p.range_start[3 * range] = first_b;
-        p.range_start[3 * range + 1] = first_row_tile;
-        p.range_start[3 * range + 2] = first_key_tile;
     }
 }
 
@@ -433,6 +435,7 @@ __global__ __launch_bounds__(256, tree_waves_per_simd(DH, NR)) void tree_keys_ke
 
     walk_range<ROWS>(p, range, kvh, [&](const TreePiece& t) {
         RowState<DH, NR> st;
+        const SequenceRows seq(p.view, t.b, kvh);
         int first_row[NR];
 #pragma unroll
         for (int n = 0; n < NR; ++n) first_row[n] = t.row0 + 16 * n;
@@ -441,7 +444,7 @@ __global__ __launch_bounds__(256, tree_waves_per_simd(DH, NR)) void tree_keys_ke
         CacheTile<DH> rk, rv; // the next tile's K and V rows, on their way
         int kt = t.key_tile + wave;
         const int first_key = (kt < t.stop_tile ? kt : t.key_tile) * kTileKeys; // (a wave without a tile: any)
-        int64_t base = p.view.key_row(t.b, first_key, kvh);
+        int64_t base = seq.key_row(first_key);
         bool odd_tiles = false;
         rk.fetch(p.view, base, first_key, t.kvlen);
         rv.fetch(p.view, base + p.view.addr.stride_kv, first_key, t.kvlen);
@@ -453,7 +456,7 @@ __global__ __launch_bounds__(256, tree_waves_per_simd(DH, NR)) void tree_keys_ke
             wave_lds_order();
             rk.stash(tile, kKeyRow<DH>, p.view.head_dim);
             wave_lds_order();
-            base = p.view.key_row(t.b, kv_next, kvh);
+            base = seq.key_row(kv_next);
             rk.fetch(p.view, base, kv_next, t.kvlen);
             float s[NR][2][4];
             uint32_t see[NR];
@@ -463,7 +466,9 @@ __global__ __launch_bounds__(256, tree_waves_per_simd(DH, NR)) void tree_keys_ke
             st.load_keys(tile, kf);
             st.scores(kf, s);
             if (!history) st.hide(p, t.s0, kv0, t.start, t.kvlen, s, see);
-            st.settle(p.scale_log2, s);
+            float top[NR];
+            st.largest(s, top);
+            if (st.passes(p.scale_log2, top)) st.settle(p.scale_log2, top);
             st.weights(p.scale_log2, s, pp);
             wave_lds_order();
             if (!history && rv.odd_rows()) {
@@ -484,7 +489,7 @@ __global__ __launch_bounds__(256, tree_waves_per_simd(DH, NR)) void tree_keys_ke
             for (kt = t.key_tile + wave; kt < t.stop_tile; kt += kTreeWaves) {
                 const int kv0 = kt * kTileKeys;
                 if (kv0 + kTileKeys <= t.start) continue;
-                base = p.view.key_row(t.b, kv0, kvh);
+                base = seq.key_row(kv0);
                 rk.fetch(p.view, base, kv0, t.kvlen);
                 rv.fetch(p.view, base + p.view.addr.stride_kv, kv0, t.kvlen);
                 wave_lds_order();
@@ -539,7 +544,7 @@ __global__ __launch_bounds__(256, tree_waves_per_simd(DH, NR)) void tree_keys_ke
                 if (t.whole) {
                     if (row < t.rows) finish_row(p, t.s0, row, kvh, channel_at<DH>(d), a, mm, l);
                 } else {
-                    const int64_t at = t.slot * ROWS + 16 * n + r;
+                    const int64_t at = (int64_t)t.slot * ROWS + 16 * n + r;
                     *reinterpret_cast<float4_t*>(p.part_o + at * DH + d) = a;
                     if (d == 0) p.part_ml[at] = make_float2(mm, l);
                 }
@@ -564,6 +569,7 @@ __global__ __launch_bounds__(W * 64, tree_waves_per_simd(DH, NB)) void tree_rows
 
     walk_range<ROWS>(p, range, kvh, [&](const TreePiece& t) {
         RowState<DH, NB> st;
+        const SequenceRows seq(p.view, t.b, kvh);
         int first_row[NB];
 #pragma unroll
         for (int n = 0; n < NB; ++n) first_row[n] = t.row0 + 16 * (wave + W * n);
@@ -571,68 +577,96 @@ __global__ __launch_bounds__(W * 64, tree_waves_per_simd(DH, NB)) void tree_rows
         const bool busy = first_row[0] < t.rows; // (a wave without rows only helps to bring the tiles)
         const int n_tiles = t.stop_tile - t.key_tile;
 
-        SharedTile<DH, W> raw[2]; // tiles i + 1 and i + 2, on their way
-        auto fetch = [&](SharedTile<DH, W>& r, int i) { // (past the last tile: that one again, so that every path has
+        // Tiles i + 1 and i + 2, on their way. Four waves bring them all, in two sets of registers by turns; eight waves in
+        // two groups, every other tile each, in the first set.
+        SharedTile<DH> raw[2];
+        const int group = W == 8 ? wave >> 2 : 0;
+        auto fetch = [&](SharedTile<DH>& r, int i) { // (past the last tile: that one again, so that every path has
                                                         // the same loads in flight and none is waited for too early)
             const int kv0 = (t.key_tile + (i < n_tiles ? i : n_tiles - 1)) * kTileKeys;
-            r.fetch(p.view, p.view.key_row(t.b, kv0, kvh), kv0, t.kvlen);
+            r.fetch(p.view, seq.key_row(kv0), kv0, t.kvlen);
         };
         bool odd_pieces = false; // this thread has kept value pieces out of the tiles
-        auto stash = [&](const SharedTile<DH, W>& r, int i) {
+        auto stash = [&](const SharedTile<DH>& r, int i) {
             const bool history = (t.key_tile + i + 1) * kTileKeys <= t.start;
             odd_pieces |= r.stash(k_lds[i & 1], v_lds[i & 1], p.view.head_dim, !history) != 0;
         };
-        uint32_t see[NB];
         __syncthreads(); // (the piece before has read its last tile)
         if (threadIdx.x == 0) odd_lds = 0;
+        // at tile i: tile i + 1 goes into LDS, tile i + 3 is requested. set: raw[(i + 1) & 1] of four waves
+        auto bring = [&](SharedTile<DH>& set, int i) {
+            if (W == 8 && group != ((i + 1) & 1)) return;
+            SharedTile<DH>& mine = W == 8 ? raw[0] : set;
+            stash(mine, i + 1);
+            fetch(mine, i + 3);
+        };
         if (n_tiles > 0) {
-            fetch(raw[0], 0);
-            fetch(raw[1], 1);
+            fetch(raw[0], group);
+            if (W == 4) fetch(raw[1], 1);
         }
         st.queries_here(p.view.head_dim);
-        __syncthreads();
-        if (n_tiles > 0) {
+        if (n_tiles > 0 && group == 0) {
             stash(raw[0], 0);
             fetch(raw[0], 2);
         }
         __syncthreads();
-        auto step = [&](SharedTile<DH, W>& next, int i) { // next: tile i + 1, then tile i + 3
+        float s[NB][2][4], top[NB];
+        // scores of tile i, while tile i + 1 goes into LDS and tile i + 3 is requested
+        auto look = [&](SharedTile<DH>& next, int i) {
             const int kv0 = (t.key_tile + i) * kTileKeys;
-            float s[NB][2][4];
-            half8_t pp[NB];
             typename RowState<DH, NB>::KeyOperands kf;
-            typename RowState<DH, NB>::ValueOperands vf;
             st.load_keys(k_lds[i & 1], kf);
-            __builtin_amdgcn_sched_barrier(0); // (the keys come out of LDS while the next tile goes in ..)
-            stash(next, i + 1);
-            fetch(next, i + 3);
+            __builtin_amdgcn_sched_barrier(0); // (the keys come out of LDS while the next tile goes in)
+            bring(next, i);
             st.scores(kf, s);
-            __builtin_amdgcn_sched_barrier(0);
-            st.load_values(v_lds[i & 1], vf); // (.. and the values, into the keys' registers, while the weights are formed)
-            __builtin_amdgcn_sched_barrier(0);
+            uint32_t see[NB];
             if (kv0 + kTileKeys > t.start) st.hide(p, t.s0, kv0, t.start, t.kvlen, s, see);
-            st.settle(p.scale_log2, s);
+            st.largest(s, top);
+        };
+        // its values
+        auto add = [&](int i) {
+            half8_t pp[NB];
+            typename RowState<DH, NB>::ValueOperands vf;
+            st.load_values(v_lds[i & 1], vf);
+            __builtin_amdgcn_sched_barrier(0); // (the values come out of LDS while the weights are formed)
             st.weights(p.scale_log2, s, pp);
             st.values(vf, pp);
             __syncthreads();
         };
         if (!busy) { // the same stashes, fetches and barriers as the others'
             for (int i = 0; i < n_tiles; ++i) {
-                if (i & 1) {
-                    stash(raw[0], i + 1);
-                    fetch(raw[0], i + 3);
-                } else {
-                    stash(raw[1], i + 1);
-                    fetch(raw[1], i + 3);
-                }
+                if (i & 1)
+                    bring(raw[0], i);
+                else
+                    bring(raw[1], i);
                 __syncthreads();
             }
         } else if (n_tiles > 0) {
-            for (int i = 0;;) { // (left from the middle, so that at its head raw[1] is always the older of the two)
-                step(raw[1], i);
-                if (++i >= n_tiles) break;
-                step(raw[0], i);
-                if (++i >= n_tiles) break;
+            int i = 0;
+            look(raw[1], 0);
+            // Reference points move out here: inside the inner loop accumulators change by matrix instructions only, and
+            // at its head raw[0] is always the older of the two tiles on their way.
+            for (bool done = false; !done;) {
+                if (st.passes(p.scale_log2, top)) st.settle(p.scale_log2, top);
+                for (;;) {
+                    add(i);
+                    done = ++i >= n_tiles;
+                    if (done) break;
+                    look(raw[0], i);
+                    if (st.passes(p.scale_log2, top)) {
+                        if (W == 4) {
+                            const SharedTile<DH> older = raw[1];
+                            raw[1] = raw[0];
+                            raw[0] = older;
+                        }
+                        break;
+                    }
+                    add(i);
+                    done = ++i >= n_tiles;
+                    if (done) break;
+                    look(raw[1], i);
+                    if (st.passes(p.scale_log2, top)) break;
+                }
             }
         }
         if (odd_pieces) odd_lds = 1;
@@ -652,14 +686,14 @@ __global__ __launch_bounds__(W * 64, tree_waves_per_simd(DH, NB)) void tree_rows
                 if (odd) atomicOr(&odd_lds, odd);
                 __syncthreads();
                 if (!busy) continue;
-                float s[NB][2][4];
+                uint32_t see[NB];
                 half8_t pp[NB];
                 typename RowState<DH, NB>::KeyOperands kf;
                 st.load_keys(k_lds[0], kf);
                 st.scores(kf, s);
                 st.hide(p, t.s0, kv0, t.start, t.kvlen, s, see);
                 st.weights(p.scale_log2, s, pp);
-                st.odd_values(p, p.view.key_row(t.b, kv0, kvh) + p.view.addr.stride_kv, kv0, t.kvlen,
+                st.odd_values(p, seq.key_row(kv0) + p.view.addr.stride_kv, kv0, t.kvlen,
                               __builtin_amdgcn_readfirstlane(odd_lds), pp, see);
             }
 #pragma unroll
@@ -677,7 +711,7 @@ __global__ __launch_bounds__(W * 64, tree_waves_per_simd(DH, NB)) void tree_rows
                         finish_row(p, t.s0, t.row0 + r, kvh, channel_at<DH>(16 * i + 4 * g), st.o[n][i],
                                    st.m[n] * p.scale_log2, l);
             } else if (st.tok[n] >= 0) {
-                const int64_t at = t.slot * ROWS + r;
+                const int64_t at = (int64_t)t.slot * ROWS + r;
 #pragma unroll
                 for (int i = 0; i < DH / 16; ++i)
                     *reinterpret_cast<float4_t*>(p.part_o + at * DH + 16 * i + 4 * g) = st.o[n][i];
