@@ -590,7 +590,7 @@ pplhip_retcode pplhip_tree_attention_forward(const pplhip_tree_attention_args* a
     bool empty;
     const pplhip_retcode rc = validate_tree(a, &empty);
     if (rc != PPLHIP_RC_SUCCESS || empty) return rc;
-    if (plan->num_ranges <= 0 || (int64_t)plan->num_ranges * a->num_kv_heads > 0x7fffffffLL ||
+    if (plan->num_ranges <= 0 || (int64_t)plan->num_ranges * a->num_kv_heads > 0x3fffffffLL ||
         plan->row_tile != tree_row_tile(a) || tree_workspace_bytes(a, plan->num_ranges) > plan->workspace_bytes)
         PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "plan was not produced by pplhip_tree_attention_prepare for these arguments");
     if (!d_workspace || ((uintptr_t)d_workspace & 255))

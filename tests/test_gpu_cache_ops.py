@@ -345,6 +345,100 @@ def test_accept_lists_end_where_they_stop_ascending():
     assert np.array_equal(cache, want_cache) and np.array_equal(scale.view(np.uint16), want_scale.view(np.uint16))
 
 
+# ---- far ends and graphs
+
+def test_everything_past_2_to_the_32_bytes():
+    """The same sequences at the far end of a slab of 4.6 GB: same outputs, bit for bit, as at the front of a small one."""
+    c = Case(8, 2, 128, [5, 12, 40], [300, 31, 900], seed=21)
+    see = trees(c)
+    near = Device(c)
+    far = Device(c)
+    torch = far.torch
+    off = 9_000_000  # tokens in front
+    first = off * c.stride_s
+    assert first > 2 ** 32
+    far.cache = torch.empty(first + c.cache.size, dtype=torch.int8, device="cuda")
+    far.scale = torch.empty(first // 8 + c.scale.size, dtype=torch.float16, device="cuda")
+    far.cache[first:] = near.cache
+    far.scale[first // 8:] = near.scale
+    far.cachestarts = near.cachestarts + off
+    n_out, n_lse = near.tree(mask_words(see, 1), 1)
+    f_out, f_lse = far.tree(mask_words(see, 1), 1)
+    assert np.array_equal(n_out, f_out) and np.array_equal(n_lse, f_lse)
+    score = c.rng.lognormal(0, 1, (1, 2, c.tokens)).astype(np.float32)
+    position = np.zeros((1, 2, c.tokens), np.int32)
+    for b in range(3):
+        position[:, :, c.tok[b]] = np.arange(c.kvlen[b])
+    pad = lambda x: np.concatenate([np.zeros((1, 2, off), x.dtype), x], axis=2)
+    pidx = c.rng.integers(0, 9999, int(c.new.sum()))
+    n_s, n_p = near.score(n_lse, score, pidx, True, position)
+    f_s, f_p = far.score(n_lse, pad(score), pidx, True, pad(position))
+    assert np.array_equal(f_s[:, :, off:], n_s) and np.array_equal(f_p[:, :, off:], n_p) and not f_s[:, :, :off].any()
+    n = near.accept([[1, 3], [0, 4], [2, 30]], [2, 2, 2], 2)[0]
+    far.accept([[1, 3], [0, 4], [2, 30]], [2, 2, 2], 2)
+    assert np.array_equal(far.cache[first:].cpu().numpy(), n)
+    near.evict(n_s, n_p, [200, 20, 500], c.kvlen, 4, 30)
+    far.evict(pad(n_s), pad(n_p), [200, 20, 500], c.kvlen, 4, 30)
+    assert np.array_equal(far.cache[first:].cpu().numpy(), near.cache.cpu().numpy())
+    assert np.array_equal(far.scale[first // 8:].cpu().numpy().view(np.uint16), near.scale.cpu().numpy().view(np.uint16))
+
+
+def test_upkeep_replays_from_a_graph():
+    """Weights, then eviction by them, captured together on a stream of their own: every replay leaves what the eager calls
+    left (the scores go to arrays of their own, so a replay finds what the first call found)."""
+    import torch
+    c = Case(8, 2, 64, [4, 9], [700, 90], seed=22)
+    lse = cache_ops.exact_attention(c, [causal(4), causal(9)])[2]
+    score, position = evict_inputs(c)
+    pidx = 2 * np.concatenate([c.old[b] + np.arange(c.new[b]) for b in range(2)])
+    want = Device(c)
+    s, p = want.score(lse, score, pidx, False, position)
+    mid = np.where(s == -5.0, score, s)
+    w_cache, w_scale, w_s, w_p, w_n = want.evict(mid, p, [300, 50], 2 * c.kvlen, 2, 40, in_place=False)
+    d = Device(c)
+    e = d.evict_args(score, position, [300, 50], 2 * c.kvlen, 2, 40, 0, 1, False)  # (holds score as d.s_in)
+    d.lse_in, d.pos_idx = d.up(lse.astype(np.float32)), d.up(pidx)
+    d.s_mid, d.pos = d.s_in.clone(), d.up(position)
+    a = d.query_args(cabi.KvScoreArgs())
+    a.d_lse, a.d_position_idx, a.d_position = d.ptr(d.lse_in), d.ptr(d.pos_idx), d.ptr(d.pos)
+    a.d_score_in, a.d_score_out = d.ptr(d.s_in), d.ptr(d.s_mid)
+    a.score_stride_l, a.score_stride_h = c.kv_heads * c.tokens, c.tokens
+    e.d_score_in, e.d_position_in = d.ptr(d.s_mid), d.ptr(d.pos)
+    plan = cabi.KvEvictPlan()
+    pkg.check(d.lib.pplhip_kv_evict_prepare(C.byref(e), C.byref(plan)))
+    ws = torch.empty(max(256, plan.workspace_bytes), dtype=torch.uint8, device="cuda")
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        st = torch.cuda.current_stream().cuda_stream
+        pkg.check(d.lib.pplhip_kv_score_accumulate(C.byref(a), st))
+        pkg.check(d.lib.pplhip_kv_evict(C.byref(e), C.byref(plan), ws.data_ptr(), st))
+    for _ in range(4):
+        d.cache.copy_(d.up(c.cache))
+        d.scale.copy_(d.up(c.scale))
+        d.s_out.fill_(-5.0)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert np.array_equal(d.cache.cpu().numpy(), w_cache)
+        assert np.array_equal(d.scale.cpu().numpy().view(np.uint16), w_scale.view(np.uint16))
+        assert np.array_equal(d.s_out.cpu().numpy(), w_s) and np.array_equal(d.p_out.cpu().numpy(), w_p)
+        assert np.array_equal(d.new_kvlen.cpu().numpy()[:2], w_n)
+
+
+@pytest.mark.parametrize("scale", [6.0, 40.0])
+def test_tree_reference_points_move_often(scale):
+    """Keys that grow along the sequence: the largest score moves up again and again, in every row at its own keys."""
+    for heads, new in ((4, 3), (8, 9), (16, 20), (32, 30), (64, 60)):
+        c = Case(heads, 1, 128, [new], [1500], seed=new)
+        c.query = (c.query * (scale / 6)).astype(np.float16)
+        r = c.rows(c.tok[0], 0, 0, 0).ravel()
+        ramp = (0.002 + 0.02 * np.linspace(0, 1, len(r))).astype(np.float16)
+        c.scale[(r // 8)[:, None] + np.arange(16)] = ramp[:, None]
+        check_tree(c, trees(c))
+
+
 # ---- together
 
 def test_speculative_steps_with_a_bounded_cache():
