@@ -8,7 +8,13 @@
 // kv_evict_choose_kernel: one workgroup per (sequence, layer, kv head). It reads the scores and positions once, as sort keys
 // into registers (up to 64 a thread), finds the K-th largest digit by digit (8 bits at a time, counts in LDS), then
 // numbers, in index order, the holes and the rows that fill them.
-// kv_evict_move_kernel: 16-byte pieces of the listed rows, K and V, with their scales.
+// kv_evict_move_kernel: 16-byte pieces of the listed rows, K and V, with their scales. One row per thread at a time and many
+// workgroups: two or four rows in flight per thread measured 53 - 61 us against 51 on the first batch below.
+//
+// Measured (KVH 8, head_dim 128): 16 sequences x 8 layers from 1 152 back to 1 024 tokens 49 us, 20 of them the choice, bound by
+// its dependent steps; the moves 2.5 TB/s (128-byte rows and 32-byte scale rows at random places). Four sequences of
+// 16 k - 64 k tokens cut to half 145 us: the choice runs on one workgroup for each of 32 columns (about 75 us), the moves
+// at 3.2 TB/s.
 #include "cache_tile.h"
 
 namespace pplhip {
@@ -295,7 +301,8 @@ pplhip_retcode launch_kv_evict(const pplhip_kv_evict_args* a, int64_t max_moves,
     p.moves = (int32_t*)ws;
     p.holes = p.moves + columns;
     p.fills = p.holes + columns * max_moves;
-    // (a column's keys fit the registers of the smallest workgroup that holds them: many short columns run side by side)
+    // A column's keys fit the registers of the smallest workgroup that holds them, so that many short columns run side by
+    // side (1 024 columns of 1 152 tokens: 54 us in all with 256 threads each, 58 with 512); long ones get all the threads.
     const dim3 cols((unsigned)columns);
     if (a->max_kvlen <= 256 * 16)
         hipLaunchKernelGGL((kv_evict_choose_kernel<256, 16>), cols, dim3(256), 0, stream, p);
@@ -324,6 +331,8 @@ pplhip_retcode launch_kv_evict(const pplhip_kv_evict_args* a, int64_t max_moves,
 // Row start + i becomes what row start + path[i] was; path is ascending, so path[i] >= i. A thread owns one 16-byte piece
 // of (layer, K or V, head) and takes the whole path through it, eight rows loaded before eight are stored: a stored
 // place (below 8 k + 8) is never a later batch's source (path[i] >= i >= 8 k + 8), and no other thread touches the piece.
+// 64 sequences with up to 6 accepted tokens, 16 layers, KVH 8, head_dim 128: 6.7 us; one sequence, 32 layers: 6.2 us; both
+// are the launch and three dependent loads.
 struct AcceptParams {
     const int64_t* seqstarts;
     const int64_t* start_pos;

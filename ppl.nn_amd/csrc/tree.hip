@@ -18,6 +18,13 @@
 // fourth key tile, through a region of LDS of its own; no barrier until the waves' shares are joined at the end of a
 // piece. tree_rows_kernel (64, 128 or 256 rows): the waves share out the rows and all read one key tile, which the whole
 // workgroup brings into LDS, so that a cached byte is dequantised once for all rows.
+//
+// What bounds it (measured, Llama-3-8B layer shape H 32 / KVH 8 / head_dim 128 unless said otherwise): 64 sequences of 4 - 16
+// drafted tokens over 256 - 4 096 keys 119 us = 3.2 TB/s, of it 10 us of partial results in the merge; 16 sequences of 64
+// tokens over 1 k - 8 k keys 116 us = 587 TFLOP/s; 8 sequences of 24 tokens over 32 k - 128 k keys at H 8 / KVH 1 141 us =
+// 531 TFLOP/s, 1.7 TB/s. Per key tile and wave (two row blocks) the vector ALU is busy for about 650 cycles (weights,
+// dequantisation), the matrix pipe for 512, LDS for 160, and the two waves a SIMD holds overlap them only in part: taking
+// out either product, the exponentials, or the staging shortens a launch by about that part's own time.
 #include "cache_tile.h"
 
 namespace pplhip {
@@ -44,8 +51,10 @@ struct TreeParams {
 };
 
 constexpr int kTreeWaves = 4; // of tree_keys_kernel
-constexpr int64_t kPieceCost = 4; // what starting and finishing a row tile costs, in key tiles
-constexpr int64_t kMinRangeTiles = 16; // a range is at least this long: four key tiles per wave of the smallest kernel
+constexpr int64_t kPieceCost = 4; // what starting and finishing a row tile costs, in key tiles (1 and 8 measure the same)
+// A range is at least this long: cutting a short axis costs the merge launch. One draft over 200 keys: 12.8 us at 8 tiles,
+// 11.2 at 16 and 32; 24 sequences of up to 1 500 keys and 20 heads: 41.4, 41.0, 51.9 us.
+constexpr int64_t kMinRangeTiles = 16;
 // The reference point m of a row's exponents need not be its running maximum: it only moves when a score passes it by
 // more than 2^kSlack, so that most tiles need neither a maximum across lanes nor a rescaling. Weights are held as
 // exp2(x - m + kProbShift), at most 2^15 in fp16 (the operand of the second product); a weight keeps fp16's full
@@ -555,7 +564,9 @@ __global__ __launch_bounds__(256, tree_waves_per_simd(DH, NR)) void tree_keys_ke
 }
 
 // W waves, each with NB blocks of 16 rows: row block i of the tile is block i / W of wave i % W, so that few rows still
-// spread over all waves. The workgroup's threads bring the key tiles into LDS, two buffers and one barrier per tile.
+// spread over all waves. The workgroup's threads bring the key tiles into LDS, two buffers and one barrier per tile. Two
+// blocks per wave, because a wave's operand reads serve both: sixteen waves of one block are bound by LDS (142 against
+// 125 us on 256 rows).
 template <int DH, int W, int NB>
 __global__ __launch_bounds__(W * 64, tree_waves_per_simd(DH, NB)) void tree_rows_kernel(const TreeParams p) {
     constexpr int ROWS = 16 * W * NB;
@@ -785,15 +796,19 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeParams p, con
 
 // ---- host side
 
-// Rows of the longest sequence's (token, shared head) pairs decide the row tile: the smallest that holds them, 256 at
-// most (128 above head_dim 128, where two row blocks' accumulators leave no room for a third wave's worth of registers).
+// The longest sequence's (token, shared head) rows decide the row tile: the smallest that holds them, so that the cache is
+// read and dequantised once; 256 at most, 128 above head_dim 128, where eight waves of two row blocks do not fit a CU's
+// registers. Measured: 64 rows in tiles of 64 / of 32 (tree_keys_kernel) 173 / 217 us on the serving batch above, 256 rows
+// in tiles of 256 / of 128 124 / 147 us, 192 rows 144 / 194 us. Up to 32 rows the other way round: tiles of 64 would leave
+// all waves but one or two without rows, where tree_keys_kernel gives each a quarter of the keys.
 int tree_row_tile(const pplhip_tree_attention_args* a) {
     const int64_t rows = a->max_seqlen * (a->num_heads / a->num_kv_heads);
     return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 || a->head_dim > 128 ? 128 : 256;
 }
 
-// As many ranges as workgroups are resident, shared out among the kv heads; never more than ranges of the least length in
-// the longest possible axis.
+// As many ranges as workgroups are resident, shared out among the kv heads (twice as many, with eight waves a workgroup:
+// 147 against 126 us on 256 rows, 203 against 171 us on 192 rows over long contexts); never more than ranges of the least
+// length in the longest possible axis.
 int64_t tree_num_ranges(const pplhip_tree_attention_args* a, int cu_count) {
     const int64_t rep = a->num_heads / a->num_kv_heads;
     const int64_t row_tiles = (a->max_seqlen * rep + tree_row_tile(a) - 1) / tree_row_tile(a);
