@@ -1,6 +1,8 @@
 """Refusals and plans of the operators that put several new tokens over the int8 slab or keep the slab up: everything
 here is decided on the host, before any device is touched."""
 import ctypes as C
+import os
+import re
 
 import pytest
 
@@ -194,3 +196,32 @@ def test_null_blocks(hiplib):
     assert hiplib.pplhip_kv_accept(None, None) == INVALID
     assert hiplib.pplhip_kv_evict_prepare(None, None) == INVALID
     assert hiplib.pplhip_tree_attention_forward(None, None, None, None) == INVALID
+
+
+@pytest.mark.parametrize("cname,cls", [
+    ("pplhip_tree_attention_args", cabi.TreeAttentionArgs), ("pplhip_tree_attention_plan", cabi.TreeAttentionPlan),
+    ("pplhip_kv_score_args", cabi.KvScoreArgs), ("pplhip_kv_evict_args", cabi.KvEvictArgs),
+    ("pplhip_kv_evict_plan", cabi.KvEvictPlan), ("pplhip_kv_accept_args", cabi.KvAcceptArgs)])
+def test_ctypes_mirrors_match_the_header(cname, cls):
+    """Names, order and types: pointers are pointers, i32 / i64 / u64 have their widths."""
+    with open(os.path.join(os.path.dirname(__file__), "..", "include", "ppl_llm_kernel_hip.h")) as f:
+        txt = re.sub(r"/\*.*?\*/", "", f.read(), flags=re.S)
+    body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (cname, cname), txt, flags=re.S).group(1)
+    want = []
+    for decl in filter(None, (d.strip() for d in body.split(";"))):
+        kind, name = decl.rsplit(None, 1)
+        if "*" in decl:
+            ctype = C.c_void_p
+        else:
+            ctype = {"int32_t": C.c_int32, "int64_t": C.c_int64, "uint64_t": C.c_uint64}[kind]
+        want.append((name.lstrip("*"), ctype))
+    assert want == list(cls._fields_)
+
+
+def test_evict_lists_that_fit_no_device(hiplib):
+    """2^31 - 1 columns of 2^31 - 1 tokens: the lists' size would pass 64 bits."""
+    a = evict()
+    a.num_kv_heads, a.layer_count, a.batch, a.max_kvlen = 1, 1, 0x7fffffff, 0x7fffffff
+    assert call(hiplib, a) == RANGE
+    a.batch = 64
+    assert call(hiplib, a) == cabi.RC_SUCCESS
