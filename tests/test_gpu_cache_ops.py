@@ -520,3 +520,56 @@ def test_speculative_steps_with_a_bounded_cache():
         n.tok = [c.cachestarts[b] + np.arange(n.kvlen[b]) for b in range(3)]
         n.cache, n.scale = cache, scale
         c, d = n, Device(n)
+
+
+def test_calls_on_two_streams_at_once():
+    """Two batches over slabs of their own: attention and eviction, a workspace each, enqueued on two streams without a
+    wait between them. Each gives what it gives alone."""
+    import torch
+    cases = [Case(32, 8, 128, [1, 9, 30], [3000, 17, 1500], seed=31), Case(8, 2, 64, [20, 3], [900, 2200], page=64, seed=32)]
+    alone, runs = [], []
+    for c in cases:
+        see, (score, position) = trees(c), evict_inputs(c)
+        upkeep = (score, position, c.kvlen // 2, 2 * c.kvlen, 2, 10)
+        d = Device(c)
+        alone.append(d.tree(mask_words(see, 1), 1) + d.evict(*upkeep))
+        d = Device(c)
+        a = d.tree_args(mask_words(see, 1), 1)
+        plan, ws = d.tree_plan(a)
+        e = d.evict_args(*upkeep, 0, c.layers, True)
+        e_plan = cabi.KvEvictPlan()
+        pkg.check(d.lib.pplhip_kv_evict_prepare(C.byref(e), C.byref(e_plan)))
+        e_ws = torch.full((max(256, e_plan.workspace_bytes),), 0xFF, dtype=torch.uint8, device="cuda")
+        runs.append((d, a, plan, ws, e, e_plan, e_ws, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for d, a, plan, ws, e, e_plan, e_ws, s in runs:
+        pkg.check(d.lib.pplhip_tree_attention_forward(C.byref(a), C.byref(plan), ws.data_ptr(), s.cuda_stream))
+    for d, a, plan, ws, e, e_plan, e_ws, s in runs:
+        pkg.check(d.lib.pplhip_kv_evict(C.byref(e), C.byref(e_plan), e_ws.data_ptr(), s.cuda_stream))
+    torch.cuda.synchronize()
+    for c, want, (d, *_) in zip(cases, alone, runs):
+        n = int(c.new.sum())
+        got = (d.out[:n], d.lse[:n], d.cache, d.scale, d.s_out, d.p_out, d.new_kvlen[:c.batch])
+        for i, (g, w) in enumerate(zip(got, want)):
+            assert g.cpu().numpy().tobytes() == w.tobytes(), i
+
+
+def test_tree_padded_batch():
+    """More rows of queries than the tables speak of (a batch padded to a fixed size, its last sequences empty) and longer
+    bounds than any sequence reaches: the same rows, nothing written behind them."""
+    c = Case(8, 2, 128, [5, 12, 0, 0], [700, 90, 0, 40], seed=33)
+    see = trees(c)
+    d = Device(c)
+    want, want_lse = d.tree(mask_words(see, 1), 1)
+    d.query = d.up(np.concatenate([c.query, np.full((47,) + c.query.shape[1:], np.nan, np.float16)]))
+    words = mask_words(see, 1)
+    a = d.tree_args(np.concatenate([words, np.full((47, 1), 2 ** 64 - 1, np.uint64)]), 1, extra_rows=47)
+    a.total_new_tokens, a.max_seqlen, a.max_kvlen = 64, 64, 4096
+    plan, ws = d.tree_plan(a)
+    pkg.check(d.lib.pplhip_tree_attention_forward(C.byref(a), C.byref(plan), ws.data_ptr(), d.stream()))
+    out, lse = d.out.cpu().numpy(), d.lse.cpu().numpy()
+    assert (out[17:] == 7.0).all() and (lse[17:] == 7.0).all()
+    ref, tol, ref_lse, lse_tol = cache_ops.exact_attention(c, see)
+    assert_within(out[:17], ref, tol, "output")
+    assert_within(lse[:17], ref_lse, lse_tol, "lse")
+    assert_within(want, ref, tol, "output of exact bounds")
