@@ -591,6 +591,8 @@ typedef struct pplhip_kv_evict_args {
     int64_t* d_new_kvlen; /* [batch] */
 } pplhip_kv_evict_args;
 
+/* Filled by pplhip_kv_evict_prepare for one argument block; prepare again when batch, max_kvlen, layer_count or
+ * num_kv_heads change. */
 typedef struct pplhip_kv_evict_plan {
     uint64_t workspace_bytes; /* device scratch the caller passes to evict, 256-byte aligned (may be 0) */
     int32_t max_moves; /* rows one (sequence, layer, kv head) can have to move: max_kvlen / 2 */
@@ -599,7 +601,7 @@ typedef struct pplhip_kv_evict_plan {
 
 /* Host-only. */
 pplhip_retcode pplhip_kv_evict_prepare(const pplhip_kv_evict_args* args, pplhip_kv_evict_plan* plan);
-/* Enqueues two launches (choice, move), allocates nothing; capturable. Overlapping calls need a workspace each. */
+/* Enqueues two launches (choice, move; six for few long sequences), allocates nothing; capturable. Overlapping calls need a workspace each. */
 pplhip_retcode pplhip_kv_evict(const pplhip_kv_evict_args* args, const pplhip_kv_evict_plan* plan, void* d_workspace,
                                void* stream);
 

@@ -631,7 +631,7 @@ static pplhip_retcode validate_evict(const pplhip_kv_evict_args* a) {
         PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "num_sink and num_recent need the tokens' positions");
     if (a->max_kvlen > 0x7fffffffLL || (double)a->batch * a->layer_count * a->num_kv_heads > 2147483647.0)
         PPLHIP_FAIL(PPLHIP_RC_OUT_OF_RANGE, "kv_evict: too many tokens or (sequence, layer, kv head) columns");
-    if ((double)a->batch * a->layer_count * a->num_kv_heads * ((double)a->max_kvlen + 2) * sizeof(int32_t) > 1e15)
+    if ((double)a->batch * a->layer_count * a->num_kv_heads * ((double)a->max_kvlen + 2) * sizeof(int32_t) > 1e12)
         PPLHIP_FAIL(PPLHIP_RC_OUT_OF_RANGE, "kv_evict: the lists of moves would not fit any device");
     if (a->batch == 0) return PPLHIP_RC_SUCCESS;
     if (!a->d_kvstarts || !a->d_cachestarts || !a->d_target_kvlen || !a->d_score_in || !a->d_score_out || !a->d_new_kvlen ||

@@ -573,3 +573,43 @@ def test_tree_padded_batch():
     assert_within(out[:17], ref, tol, "output")
     assert_within(lse[:17], ref_lse, lse_tol, "lse")
     assert_within(want, ref, tol, "output of exact bounds")
+
+
+@pytest.mark.parametrize("ties,nan", [(False, False), (True, False), (False, True), (True, True)])
+@pytest.mark.parametrize("in_place", [True, False])
+def test_evict_long_beside_short(ties, nan, in_place):
+    """A column several workgroups share beside columns of one of their parts, of a few tokens and of none; some keep
+    everything, nothing, or all but one."""
+    kv = [20000, 4096, 4097, 3, 0, 8192, 17000, 16500]
+    keep = [9000, 100, 4097, 1, 0, 8191, 0, 20000]
+    check_evict(Case(2, 2, 16, [1 if n else 0 for n in kv], [max(0, n - 1) for n in kv], layers=2, page=64, seed=34), keep,
+                sinks=3, recent=100, in_place=in_place, ties=ties, nan=nan)
+
+
+@pytest.mark.parametrize("n,keep", [(65536, 40000), (65537, 30000), (262144, 262143), (262145, 131072), (300000, 1)])
+def test_evict_longest(n, keep):
+    """Either side of where a workgroup's registers, and the largest number of one-block parts, end."""
+    check_evict(Case(1, 1, 16, [1], [n - 1], seed=35), [keep], sinks=4, recent=1000)
+
+
+def test_evict_many_long_columns():
+    """147 columns: each longer than 16 384 tokens, and more than several workgroups a column pay for."""
+    check_evict(Case(7, 7, 16, [1, 1, 1], [17000, 20001, 900], layers=7, seed=36), [16900, 19999, 850], sinks=4, recent=64)
+
+
+def test_evict_longer_than_announced():
+    """A table that speaks of more tokens than max_kvlen: the first max_kvlen are looked at, the rest left alone."""
+    c = Case(2, 2, 16, [1], [999], seed=37)
+    score, position = evict_inputs(c)
+    d = Device(c)
+    a = d.evict_args(score, position, [300], [2000], 0, 0, 0, 1, True)
+    a.max_kvlen = 600
+    plan = cabi.KvEvictPlan()
+    pkg.check(d.lib.pplhip_kv_evict_prepare(C.byref(a), C.byref(plan)))
+    ws = d.torch.empty(plan.workspace_bytes, dtype=d.torch.uint8, device="cuda")
+    pkg.check(d.lib.pplhip_kv_evict(C.byref(a), C.byref(plan), ws.data_ptr(), d.stream()))
+    c.kvlen[0] = 600
+    c.tok[0] = c.tok[0][:600]
+    e_cache, e_scale, e_s, e_p, e_n = cache_ops.exact_evict(c, score, position, [300], [2000], 0, 0, 0, 1)
+    assert np.array_equal(d.cache.cpu().numpy(), e_cache) and np.array_equal(d.s_out.cpu().numpy(), e_s)
+    assert np.array_equal(d.p_out.cpu().numpy(), e_p) and int(d.new_kvlen[0]) == 300
