@@ -8,7 +8,7 @@
 // The choice: scores and positions are read once, as sort keys; the K-th largest is found digit by digit (8 bits at a time,
 // counts in LDS); then the holes and the rows that fill them are numbered in index order. kv_evict_choose_kernel does it
 // with one workgroup per (sequence, layer, kv head), keys in registers (up to 64 a thread); kv_evict_digit_kernel and
-// kv_evict_number_kernel with several, where columns are long and few.
+// kv_evict_number_kernel with several, where columns are long and few, or too long for registers.
 // kv_evict_move_kernel: 16-byte pieces of the listed rows, K and V, with their scales. One row per thread at a time and many
 // workgroups: two or four rows in flight per thread measured 53 - 61 us against 51 on the first batch below.
 //
