@@ -601,7 +601,8 @@ typedef struct pplhip_kv_evict_plan {
 
 /* Host-only. */
 pplhip_retcode pplhip_kv_evict_prepare(const pplhip_kv_evict_args* args, pplhip_kv_evict_plan* plan);
-/* Enqueues two launches (choice, move; six where max_kvlen is large), allocates nothing; capturable. Overlapping calls need a workspace each. */
+/* Enqueues two launches (choice, move; six where max_kvlen is large), allocates nothing; capturable. Overlapping calls
+ * need a workspace each. */
 pplhip_retcode pplhip_kv_evict(const pplhip_kv_evict_args* args, const pplhip_kv_evict_plan* plan, void* d_workspace,
                                void* stream);
 
