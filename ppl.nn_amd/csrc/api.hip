@@ -578,8 +578,10 @@ pplhip_retcode pplhip_tree_attention_prepare(const pplhip_tree_attention_args* a
     bool empty;
     const pplhip_retcode rc = validate_tree(a, &empty);
     if (rc != PPLHIP_RC_SUCCESS || empty) return rc;
+    const int64_t ranges = tree_num_ranges(a, device_cu_count());
+    if (!tree_launches_fit(a, ranges)) PPLHIP_FAIL(PPLHIP_RC_OUT_OF_RANGE, "too many kv heads for a launch");
     plan->row_tile = tree_row_tile(a);
-    plan->num_ranges = (int32_t)tree_num_ranges(a, device_cu_count());
+    plan->num_ranges = (int32_t)ranges;
     plan->workspace_bytes = (tree_workspace_bytes(a, plan->num_ranges) + 255) / 256 * 256;
     return PPLHIP_RC_SUCCESS;
 }
@@ -590,8 +592,8 @@ pplhip_retcode pplhip_tree_attention_forward(const pplhip_tree_attention_args* a
     bool empty;
     const pplhip_retcode rc = validate_tree(a, &empty);
     if (rc != PPLHIP_RC_SUCCESS || empty) return rc;
-    if (plan->num_ranges <= 0 || (int64_t)plan->num_ranges * a->num_kv_heads > 0x3fffffffLL ||
-        plan->row_tile != tree_row_tile(a) || tree_workspace_bytes(a, plan->num_ranges) > plan->workspace_bytes)
+    if (plan->num_ranges <= 0 || plan->row_tile != tree_row_tile(a) || !tree_launches_fit(a, plan->num_ranges) ||
+        tree_workspace_bytes(a, plan->num_ranges) > plan->workspace_bytes)
         PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "plan was not produced by pplhip_tree_attention_prepare for these arguments");
     if (!d_workspace || ((uintptr_t)d_workspace & 255))
         PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "workspace of %llu bytes (256-byte aligned) required",
@@ -631,6 +633,7 @@ static pplhip_retcode validate_evict(const pplhip_kv_evict_args* a) {
         PPLHIP_FAIL(PPLHIP_RC_INVALID_VALUE, "num_sink and num_recent need the tokens' positions");
     if (a->max_kvlen > 0x7fffffffLL || (double)a->batch * a->layer_count * a->num_kv_heads > 2147483647.0)
         PPLHIP_FAIL(PPLHIP_RC_OUT_OF_RANGE, "kv_evict: too many tokens or (sequence, layer, kv head) columns");
+    if (!evict_launches_fit(a)) PPLHIP_FAIL(PPLHIP_RC_OUT_OF_RANGE, "kv_evict: too many columns for a launch");
     if ((double)a->batch * a->layer_count * a->num_kv_heads * ((double)a->max_kvlen + 2) * sizeof(int32_t) > 1e12)
         PPLHIP_FAIL(PPLHIP_RC_OUT_OF_RANGE, "kv_evict: the lists of moves would not fit any device");
     if (a->batch == 0) return PPLHIP_RC_SUCCESS;

@@ -26,6 +26,11 @@ void set_error(const char* fmt, ...) __attribute__((format(printf, 1, 2)));
             PPLHIP_FAIL(PPLHIP_RC_DEVICE_RUNTIME_ERROR, "%s: %s", (what), hipGetErrorString(e_)); \
     } while (0)
 
+// A launch has less than 2^32 threads along an axis of its grid. In double, so that no count overflows on the way here.
+inline bool launch_fits(double workgroups, int threads) {
+    return workgroups * threads <= 4294967295.0;
+}
+
 constexpr int kQuantGroup = 8;
 constexpr int kWave = 64;
 
@@ -207,10 +212,12 @@ void check_tables_host(const pplhip_mhca_args* a, int64_t max_slab_tokens, int32
 // several new tokens per sequence over the slab (tree.hip); the plan's ranges, row tile and workspace
 int tree_row_tile(const pplhip_tree_attention_args* a);
 int64_t tree_num_ranges(const pplhip_tree_attention_args* a, int cu_count);
+bool tree_launches_fit(const pplhip_tree_attention_args* a, int64_t ranges);
 uint64_t tree_workspace_bytes(const pplhip_tree_attention_args* a, int64_t ranges);
 pplhip_retcode launch_tree_attention(const pplhip_tree_attention_args* a, int64_t ranges, void* ws, hipStream_t stream);
 pplhip_retcode launch_kv_score(const pplhip_kv_score_args* a, hipStream_t stream);
 // eviction and accepted drafts (evict.hip)
+bool evict_launches_fit(const pplhip_kv_evict_args* a);
 uint64_t evict_workspace_bytes(const pplhip_kv_evict_args* a, int64_t max_moves);
 pplhip_retcode launch_kv_evict(const pplhip_kv_evict_args* a, int64_t max_moves, void* ws, hipStream_t stream);
 pplhip_retcode launch_kv_accept(const pplhip_kv_accept_args* a, hipStream_t stream);

@@ -456,6 +456,9 @@ int64_t evict_columns(const pplhip_kv_evict_args* a) {
 //   65 536         64 / 31   70 / 42   73 / 55   76 / 86   87 / 140
 // (131 072 tokens read anew for every digit by one workgroup each: 242 / 35 one column, 306 / 257 with 256.)
 constexpr int64_t kEvictSplitAbove = 16384, kEvictRegisterKeys = 65536, kEvictSplitColumns = 96;
+static bool evict_split(int64_t max_kvlen, double columns) {
+    return max_kvlen > kEvictRegisterKeys || (max_kvlen > kEvictSplitAbove && columns <= (double)kEvictSplitColumns);
+}
 // Parts of a column: at most kEvictParts, of whole blocks.
 constexpr int kEvictParts = 64;
 int64_t evict_part_blocks(int64_t max_kvlen) {
@@ -464,6 +467,12 @@ int64_t evict_part_blocks(int64_t max_kvlen) {
 int64_t evict_parts(int64_t max_kvlen) {
     const int64_t tokens = evict_part_blocks(max_kvlen) * kPartBlock;
     return tokens ? (max_kvlen + tokens - 1) / tokens : 0;
+}
+// the largest of a call's launches: the choice (the moves' has 256 threads a column, or few)
+bool evict_launches_fit(const pplhip_kv_evict_args* a) {
+    const double columns = (double)a->batch * a->layer_count * a->num_kv_heads;
+    if (evict_split(a->max_kvlen, columns)) return launch_fits(columns * (double)evict_parts(a->max_kvlen), 256);
+    return launch_fits(columns, a->max_kvlen > 256 * 16 ? 1024 : 256);
 }
 uint64_t evict_workspace_bytes(const pplhip_kv_evict_args* a, int64_t max_moves) {
     uint64_t ints = 1 + 2 * (uint64_t)max_moves;
@@ -499,7 +508,7 @@ pplhip_retcode launch_kv_evict(const pplhip_kv_evict_args* a, int64_t max_moves,
     p.part_blocks = (int32_t)evict_part_blocks(a->max_kvlen);
     p.parts = (int32_t)evict_parts(a->max_kvlen);
     p.keys = (uint4_vt*)ws;
-    const bool split = a->max_kvlen > kEvictRegisterKeys || (a->max_kvlen > kEvictSplitAbove && columns <= kEvictSplitColumns);
+    const bool split = evict_split(a->max_kvlen, (double)columns);
     p.moves = (int32_t*)ws + (split ? columns * p.parts * p.part_blocks * kPartBlock : 0);
     p.holes = p.moves + columns;
     p.fills = p.holes + columns * max_moves;
@@ -629,9 +638,11 @@ pplhip_retcode launch_kv_accept(const pplhip_kv_accept_args* a, hipStream_t stre
     p.layer_count = a->layer_count;
     p.kv_heads = a->num_kv_heads;
     p.pieces = a->head_dim / 16;
+    // (in double first: the product can pass 64 bits)
+    const double blocks = ceil((double)a->layer_count * 2.0 * a->num_kv_heads * p.pieces / 256.0) * (double)a->batch;
+    if (!launch_fits(blocks, 256)) PPLHIP_FAIL(PPLHIP_RC_OUT_OF_RANGE, "kv_accept: too many rows");
     const int64_t units = (int64_t)a->layer_count * 2 * a->num_kv_heads * p.pieces;
     const int64_t per_seq = (units + 255) / 256;
-    if (per_seq * a->batch > 0x7fffffffLL) PPLHIP_FAIL(PPLHIP_RC_OUT_OF_RANGE, "kv_accept: too many rows");
     p.blocks_per_seq = (int32_t)per_seq;
     hipLaunchKernelGGL(kv_accept_kernel, dim3((unsigned)(per_seq * a->batch)), dim3(256), 0, stream, p);
     PPLHIP_CHECK_LAUNCH("kv_accept");

@@ -190,7 +190,7 @@ pplhip_retcode launch_kv_score(const pplhip_kv_score_args* a, hipStream_t stream
     p.rep = a->num_heads / a->num_kv_heads;
     p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)a->head_dim));
     const int64_t key_blocks = (a->max_kvlen + kScoreKeys - 1) / kScoreKeys;
-    if ((double)key_blocks * (double)a->batch * (double)a->num_kv_heads > 2147483647.0)
+    if (!launch_fits((double)key_blocks * (double)a->batch * (double)a->num_kv_heads, 256))
         PPLHIP_FAIL(PPLHIP_RC_OUT_OF_RANGE, "kv_score: too many key blocks");
     p.key_blocks = (int32_t)key_blocks;
     const dim3 grid((unsigned)(key_blocks * a->batch * a->num_kv_heads));

@@ -821,6 +821,10 @@ int64_t tree_num_ranges(const pplhip_tree_attention_args* a, int cu_count) {
     return ranges < 1 ? 1 : ranges;
 }
 
+bool tree_launches_fit(const pplhip_tree_attention_args* a, int64_t ranges) {
+    return launch_fits((double)ranges * a->num_kv_heads, tree_row_tile(a) == 256 ? 512 : 256);
+}
+
 uint64_t tree_workspace_bytes(const pplhip_tree_attention_args* a, int64_t ranges) {
     const uint64_t rows = (uint64_t)a->num_kv_heads * 2 * (uint64_t)ranges * tree_row_tile(a);
     return rows * padded_head_dim(a->head_dim) * sizeof(float) + rows * sizeof(float2) + (uint64_t)ranges * 3 * sizeof(int64_t);

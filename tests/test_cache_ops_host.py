@@ -225,3 +225,42 @@ def test_evict_lists_that_fit_no_device(hiplib):
     assert call(hiplib, a) == RANGE
     a.batch = 64
     assert call(hiplib, a) == cabi.RC_SUCCESS
+
+
+def many_heads(a, heads):
+    a.num_heads = a.num_kv_heads = heads
+    return a
+
+
+def test_launches_of_2_to_the_32_threads(hiplib):
+    """A launch has less than 2^32 threads along its axis: what would need more is refused before anything is enqueued
+    (of the calls that would enqueue only the refused side is looked at), by prepare as well."""
+    a = score()  # 512 blocks of keys x 4096 sequences x 8 kv heads = 2^24 workgroups of 256
+    a.max_kvlen, a.batch = 131072, 4096
+    assert call(hiplib, a) == RANGE
+    a = accept()  # two workgroups a sequence
+    a.layer_idx, a.layer_count, a.batch = 0, 4, 1 << 23
+    assert call(hiplib, a) == RANGE
+    a = accept()  # (the rows' count itself would pass 64 bits)
+    a.layer_idx, a.layer_count, a.num_layer, a.num_kv_heads = 0, 0x7fffffff, 0x7fffffff, 0x7fffffff
+    assert call(hiplib, a) == RANGE
+    # columns: 16 a sequence; workgroups of 256 and 1024 threads, and 17 of 256 a column
+    for kvlen, batch in ((500, 1 << 20), (5000, 1 << 18), (20000, 1 << 18), (65537, 61681)):
+        a = evict()
+        a.max_kvlen, a.batch = kvlen, batch
+        assert call(hiplib, a) == RANGE, kvlen
+        a.batch -= 1
+        assert call(hiplib, a) == cabi.RC_SUCCESS, kvlen
+    # one range: workgroups of 256 threads, of 512 for tiles of 256 rows
+    for seqlen, heads in ((10, 1 << 24), (200, 1 << 23)):
+        a = many_heads(tree(), heads)
+        a.total_new_tokens = a.max_seqlen = seqlen
+        a.d_tree_mask = None
+        assert call(hiplib, a) == RANGE, seqlen
+        assert call(hiplib, many_heads(a, heads - 1)) == cabi.RC_SUCCESS, seqlen
+    plan = cabi.TreeAttentionPlan()  # a plan of more ranges than prepare would make
+    a = tree()
+    assert call(hiplib, a, plan) == cabi.RC_SUCCESS
+    big = cabi.TreeAttentionPlan(1 << 62, 1 << 21, plan.row_tile)
+    assert hiplib.pplhip_tree_attention_forward(C.byref(a), C.byref(big), None, None) == INVALID
+    assert b"plan" in hiplib.pplhip_last_error()
