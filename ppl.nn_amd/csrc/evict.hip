@@ -474,11 +474,17 @@ bool evict_launches_fit(const pplhip_kv_evict_args* a) {
     if (evict_split(a->max_kvlen, columns)) return launch_fits(columns * (double)evict_parts(a->max_kvlen), 256);
     return launch_fits(columns, a->max_kvlen > 256 * 16 ? 1024 : 256);
 }
+// (a plan for many columns holds what fewer of them take, which several workgroups share)
 uint64_t evict_workspace_bytes(const pplhip_kv_evict_args* a, int64_t max_moves) {
-    uint64_t ints = 1 + 2 * (uint64_t)max_moves;
-    if (a->max_kvlen > kEvictSplitAbove)
-        ints += 8 + (uint64_t)evict_parts(a->max_kvlen) * (513 + kPartBlock * (uint64_t)evict_part_blocks(a->max_kvlen));
-    return (uint64_t)evict_columns(a) * ints * sizeof(int32_t);
+    const uint64_t columns = (uint64_t)evict_columns(a), lists = 1 + 2 * (uint64_t)max_moves;
+    uint64_t ints = columns * lists;
+    if (a->max_kvlen > kEvictSplitAbove) {
+        const uint64_t shared = evict_split(a->max_kvlen, (double)columns) ? columns : kEvictSplitColumns;
+        const uint64_t each = lists + 8 + (uint64_t)evict_parts(a->max_kvlen) *
+                                              (513 + kPartBlock * (uint64_t)evict_part_blocks(a->max_kvlen));
+        if (shared * each > ints) ints = shared * each;
+    }
+    return ints * sizeof(int32_t);
 }
 
 pplhip_retcode launch_kv_evict(const pplhip_kv_evict_args* a, int64_t max_moves, void* ws, hipStream_t stream) {

@@ -264,3 +264,24 @@ def test_launches_of_2_to_the_32_threads(hiplib):
     big = cabi.TreeAttentionPlan(1 << 62, 1 << 21, plan.row_tile)
     assert hiplib.pplhip_tree_attention_forward(C.byref(a), C.byref(big), None, None) == INVALID
     assert b"plan" in hiplib.pplhip_last_error()
+
+
+@pytest.mark.parametrize("kvlen", [16385, 40000, 65536])
+def test_evict_workspace_holds_what_the_call_uses(hiplib, kvlen):
+    """Up to 96 columns several workgroups choose from one and keep its keys in the workspace; above that, up to 65 536
+    tokens, one does, and only the lists of moves (their count, holes, fillers) are there. A plan for a large batch also
+    serves a smaller one, whose columns are shared."""
+    a, plan = evict(), cabi.KvEvictPlan()
+    a.max_kvlen, a.num_layer, a.layer_idx, a.layer_count, a.num_kv_heads, a.batch = kvlen, 1, 0, 1, 1, 96
+    lists = lambda columns: -(-columns * (1 + 2 * (kvlen // 2)) * 4 // 256) * 256
+    assert call(hiplib, a, plan) == cabi.RC_SUCCESS
+    shared = plan.workspace_bytes
+    assert shared >= lists(96) + 96 * kvlen * 4
+    for columns in (97, 150, 4096):
+        a.batch = columns
+        assert call(hiplib, a, plan) == cabi.RC_SUCCESS
+        assert plan.workspace_bytes == max(shared, lists(columns))
+        for fewer in (1, 96, 97):
+            a.batch = min(fewer, columns)
+            assert hiplib.pplhip_kv_evict(C.byref(a), C.byref(plan), None, None) == INVALID
+            assert b"workspace" in hiplib.pplhip_last_error()  # not the plan
