@@ -613,3 +613,124 @@ def test_evict_longer_than_announced():
     e_cache, e_scale, e_s, e_p, e_n = cache_ops.exact_evict(c, score, position, [300], [2000], 0, 0, 0, 1)
     assert np.array_equal(d.cache.cpu().numpy(), e_cache) and np.array_equal(d.s_out.cpu().numpy(), e_s)
     assert np.array_equal(d.p_out.cpu().numpy(), e_p) and int(d.new_kvlen[0]) == 300
+
+
+# ---- every kernel at every padded head size
+
+HEAD_DIMS = list(range(16, 257, 16))
+
+
+@pytest.mark.parametrize("rows", [16, 17, 33, 65, 129, 257])
+@pytest.mark.parametrize("dim", HEAD_DIMS)
+def test_tree_row_tiles(dim, rows):
+    """Row counts that select each row tile, one more than a tile holds among them, at every head size: by mask, causal."""
+    c = Case(2, 2, dim, [rows, rows // 2, 1], [45, 0, 130], seed=1000 * dim + rows)
+    check_tree(c, trees(c), junk=True)
+    check_tree(c)
+
+
+def spoil(c, b, new_token, bits, kv=slice(None)):
+    """Gives the scales of a new token's rows these fp16 bits."""
+    r = c.rows(c.tok[b][c.old[b] + new_token], c.layer, slice(None), kv).ravel()
+    c.scale.view(np.uint16)[(r // 8)[:, None] + np.arange(c.dim // 8)] = bits
+
+
+@pytest.mark.parametrize("rows", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("dim", HEAD_DIMS)
+def test_tree_hidden_tokens_in_every_row_tile(dim, rows):
+    """Tokens that nobody else sees with NaN and infinite scales, one that sees itself, and one with values near fp16's
+    largest that others do see; a sequence without history and one whose new tokens share a key tile with it."""
+    c = Case(2, 2, dim, [rows, rows, 3], [0, 50, 9], seed=1000 * dim + rows)
+    see = trees(c)
+    for b in (0, 1):
+        for x, bits in ((3, 0x7E00), (rows // 2, 0x7C00), (rows - 1, 0xFC00)):
+            see[b][:, x] = False
+            spoil(c, b, x, bits)
+        see[b][3, 3] = True
+        spoil(c, b, 5, np.float16(514.0).view(np.uint16), 1)
+    got, _ = check_tree(c, see)
+    assert np.isnan(got[3]).all() and np.isfinite(np.delete(got, [3, rows + 3], axis=0)).all()
+
+
+@pytest.mark.parametrize("rows", [5, 20, 50, 100, 200])
+def test_tree_infinite_values_that_are_seen(rows):
+    """An infinite value row, in front of the new tokens and among them, reaches those that see it, with its signs."""
+    c = Case(2, 1, 128, [rows], [100], seed=rows)
+    c.cache[c.cache == 0] = 1  # (0 times infinity has no sign)
+    see = trees(c)
+    spoil(c, 0, 4, 0x7C00, 1)
+    check_tree(c, see)
+    spoil(c, 0, -37, 0x7C00, 1)
+    got, _ = check_tree(c, see)
+    assert not np.isfinite(got).any()
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 64), (4, 1, 128), (2, 2, 256), (3, 3, 80)])
+def test_tree_whole_prompts(heads, kv_heads, dim):
+    c = Case(heads, kv_heads, dim, [600, 1, 333], [0, 50, 77], seed=dim)
+    check_tree(c)
+
+
+@pytest.mark.parametrize("dim", HEAD_DIMS)
+def test_score_head_dims(dim):
+    check_score(Case(4, 2, dim, [5, 1, 0, 70], [70, 0, 20, 300], seed=dim))
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 64), (3, 3, 192)])
+def test_score_whole_prompts(heads, kv_heads, dim):
+    check_score(Case(heads, kv_heads, dim, [600, 333], [0, 77], seed=dim))
+
+
+@pytest.mark.parametrize("columns", [96, 97])
+def test_evict_long_without_positions(columns):
+    """Either side of where several workgroups choose from a long column."""
+    c = Case(1, 1, 16, [1] * columns, [17000] + [200] * (columns - 1), seed=columns)
+    check_evict(c, [9000] + [100] * (columns - 1), positions=False)
+
+
+def test_score_padded_batch():
+    """Rows behind the last sequence hold NaN, the last sequences are empty, the bounds are longer than any sequence."""
+    c = Case(8, 2, 128, [5, 130, 0, 0], [700, 90, 0, 40], seed=61)
+    lse = cache_ops.exact_attention(c, [causal(int(n)) for n in c.new])[2].astype(np.float32)
+    score = np.abs(c.rng.standard_normal((1, 2, c.tokens))).astype(np.float32)
+    want, want_pos = Device(c).score(lse, score, np.arange(135), False, np.full(score.shape, -3, np.int32))
+    d = Device(c)
+    d.query = d.up(np.concatenate([c.query, np.full((57,) + c.query.shape[1:], np.nan, np.float16)]))
+    a = d.query_args(cabi.KvScoreArgs())
+    a.total_new_tokens, a.max_seqlen, a.max_kvlen = 192, 192, 4096
+    lse_dev = d.up(np.concatenate([lse, np.full((57, 8), np.nan, np.float32)]))
+    s_in, s_out = d.up(score), d.up(np.full_like(score, -5.0))
+    idx, pos = d.up(np.concatenate([np.arange(135), np.full(57, -9)])), d.up(np.full(score.shape, -3, np.int32))
+    a.d_lse, a.d_position_idx, a.d_position = d.ptr(lse_dev), d.ptr(idx), d.ptr(pos)
+    a.d_score_in, a.d_score_out = d.ptr(s_in), d.ptr(s_out)
+    a.score_stride_l, a.score_stride_h = 2 * c.tokens, c.tokens
+    pkg.check(d.lib.pplhip_kv_score_accumulate(C.byref(a), d.stream()))
+    assert np.array_equal(s_out.cpu().numpy(), want) and np.array_equal(pos.cpu().numpy(), want_pos)
+
+
+@pytest.mark.parametrize("n", [700, 17000])
+@pytest.mark.parametrize("scores_in_place", [True, False])
+def test_evict_one_of_scores_and_positions_in_place(n, scores_in_place):
+    c = Case(2, 2, 16, [1, 1], [n - 1, 50], seed=n)
+    score, position = evict_inputs(c)
+    keep = [n // 3, 20]
+    d = Device(c)
+    a = d.evict_args(score, position, keep, 2 * c.kvlen, 2, 30, 0, 1, False)
+    if scores_in_place:
+        a.d_score_out = a.d_score_in
+    else:
+        a.d_position_out = a.d_position_in
+    plan = cabi.KvEvictPlan()
+    pkg.check(d.lib.pplhip_kv_evict_prepare(C.byref(a), C.byref(plan)))
+    ws = d.torch.full((plan.workspace_bytes,), 0xFF, dtype=d.torch.uint8, device="cuda")
+    pkg.check(d.lib.pplhip_kv_evict(C.byref(a), C.byref(plan), ws.data_ptr(), d.stream()))
+    e_cache, e_scale, e_s, e_p, e_n = cache_ops.exact_evict(c, score, position, keep, 2 * c.kvlen, 2, 30, 0, 1)
+    assert np.array_equal(d.cache.cpu().numpy(), e_cache)
+    got_s, got_p = (d.s_in, d.p_out) if scores_in_place else (d.s_out, d.p_in)
+    for b in range(2):
+        t = c.tok[b][:int(e_n[b])]
+        assert np.array_equal(got_s.cpu().numpy()[:, :, t], e_s[:, :, t])
+        assert np.array_equal(got_p.cpu().numpy()[:, :, t], e_p[:, :, t])
+        t = c.tok[b][int(e_n[b]):]
+        same = (got_s, score) if scores_in_place else (got_p, position)
+        assert np.array_equal(same[0].cpu().numpy()[:, :, t], same[1][:, :, t])
