@@ -442,6 +442,8 @@ pplhip_retcode pplhip_check_tables_host(const pplhip_mhca_args* args, int64_t ma
  * pplhip_rope_kv_write_forward put them there). A token sees every cached token in front of the new ones, and of the
  * new ones those its mask row names; score = q . k / sqrt(head_dim). A row that sees nothing yields zeros and -inf.
  * Keys a row does not see contribute nothing to it, whatever the slab holds for them (NaN and infinities included).
+ * Scores, their maxima and sums and the outputs' sums are fp32; the softmax weights are rounded to fp16 before they meet
+ * the values (a relative 2^-11 of each), lse does not depend on that.
  * Rows of query / output at or past seqstarts[batch] are neither read nor written.
  * head_dim: a multiple of 16 up to 256; any num_heads that num_kv_heads divides; cache layouts, pages and strides as
  * for pplhip_mhca_args. Drafted tokens' rotary positions (start + depth in the tree) are not those of a run of
@@ -545,7 +547,8 @@ pplhip_retcode pplhip_kv_score_accumulate(const pplhip_kv_score_args* args, void
 
 /*
  * Eviction from the cache by accumulated attention weight. For every sequence b, layer layer_idx .. layer_idx +
- * layer_count - 1 and kv head on its own, K = min(kvlen, max(target_kvlen[b], 0)) of the kvlen cached tokens stay:
+ * layer_count - 1 and kv head on its own, K = min(kvlen, max(target_kvlen[b], 0)) of the kvlen cached tokens stay
+ * (a sequence of more than max_kvlen tokens counts as one of max_kvlen: those behind are dropped, whatever their scores):
  * first those whose position is below num_sink or at least next_pos[b] - num_recent, then those with the largest score;
  * a NaN score counts as the smallest, ties go to the lower index. Tokens with index below K that stay are left where
  * they are; the j-th token (ascending) with index below K that goes has its slab row (int8 K and V, scales, score,
@@ -601,8 +604,8 @@ typedef struct pplhip_kv_evict_plan {
 
 /* Host-only. */
 pplhip_retcode pplhip_kv_evict_prepare(const pplhip_kv_evict_args* args, pplhip_kv_evict_plan* plan);
-/* Enqueues two launches (choice, move; six where max_kvlen is large), allocates nothing; capturable. Overlapping calls
- * need a workspace each. */
+/* Enqueues two launches (choice, move), six where max_kvlen is above 65 536, or above 16 384 with at most 96 (sequence,
+ * layer, kv head) columns; allocates nothing; capturable. Overlapping calls need a workspace each. */
 pplhip_retcode pplhip_kv_evict(const pplhip_kv_evict_args* args, const pplhip_kv_evict_plan* plan, void* d_workspace,
                                void* stream);
 
