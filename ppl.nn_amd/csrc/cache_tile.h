@@ -8,8 +8,10 @@
 // In LDS a row has DH channels (head_dim rounded up to a multiple of 32, zeros past head_dim) in units of one group (16
 // bytes): first the pieces' even groups, then their odd ones, so that the lanes of a row write 16 consecutive units at a
 // time. Which channel a position holds (channel_at) only matters where queries are loaded and outputs stored. K rows are
-// padded by one unit, V rows by two: the 16-byte reads of 16 K rows at one position, and the transposing 8-byte reads of
-// four V rows, then touch every bank once.
+// padded by one unit, V rows by two, so that the 16-byte reads of 16 K rows at one position, and the transposing 8-byte reads
+// of four V rows, touch every bank once. Lanes of other positions come in between: the counter of bank conflicts has 32
+// cycles per tile of 128 channels and wave that reads it (in tree.hip of some 110 that LDS is busy for), and none that go
+// with the stores.
 #ifndef PPLHIP_CSRC_CACHE_TILE_H_
 #define PPLHIP_CSRC_CACHE_TILE_H_
 

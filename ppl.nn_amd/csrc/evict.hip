@@ -12,9 +12,9 @@
 // kv_evict_move_kernel: 16-byte pieces of the listed rows, K and V, with their scales. One row per thread at a time and many
 // workgroups: two or four rows in flight per thread measured 53 - 61 us against 51 on the first batch below.
 //
-// Measured (KVH 8, head_dim 128): 16 sequences x 8 layers from 1 152 back to 1 024 tokens 47 us, 18 of them the choice, bound by
-// its dependent steps; the moves 2.5 TB/s (128-byte rows and 32-byte scale rows at random places). Four sequences of
-// 16 k - 64 k tokens cut to half, one layer: 110 us, about 50 of them the choice, mostly its five launches, each a chain of
+// Measured (KVH 8, head_dim 128): 16 sequences x 8 layers from 1 152 back to 1 024 tokens 47 us, 18 of them the choice, bound
+// by its dependent steps; the moves 2.5 TB/s (128-byte rows and 32-byte scale rows at random places). Four sequences of
+// 16 k - 64 k tokens cut to half, one layer: 110 us, 45 of them the choice, mostly its five launches, each a chain of
 // dependent loads (one workgroup for each of the 32 columns: 141); the moves at 3.2 TB/s.
 #include "cache_tile.h"
 
@@ -561,7 +561,7 @@ pplhip_retcode launch_kv_evict(const pplhip_kv_evict_args* a, int64_t max_moves,
 // of (layer, K or V, head) and takes the whole path through it, eight rows loaded before eight are stored: a stored
 // place (below 8 k + 8) is never a later batch's source (path[i] >= i >= 8 k + 8), and no other thread touches the piece.
 // 64 sequences with up to 6 accepted tokens, 16 layers, KVH 8, head_dim 128: 6.7 us; one sequence, 32 layers: 6.2 us; both
-// are the launch and three dependent loads.
+// are three dependent loads (the list's length, the list, the rows) and a store in one launch.
 struct AcceptParams {
     const int64_t* seqstarts;
     const int64_t* start_pos;

@@ -10,7 +10,7 @@
 //
 // One row block (a decode step) is bound by memory: 64 sequences of 256 - 4 096 keys, H 32 / KVH 8 / head_dim 128, 50.6 us =
 // 3.7 TB/s. Windows of queries are bound by the exponentials and the start of a workgroup (keys, then rows, before the
-// first product): 32 queries over 4 k - 32 k keys of 8 sequences 65 us = 465 TFLOP/s, 2.4 TB/s. Requesting the rows
+// first product): 32 queries over 4 k - 32 k keys of 8 sequences 65 us = 463 TFLOP/s, 2.4 TB/s. Requesting the rows
 // together with the keys costs registers, and with them half the waves: 81 us.
 #include "cache_tile.h"
 

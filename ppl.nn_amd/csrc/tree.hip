@@ -19,12 +19,14 @@
 // piece. tree_rows_kernel (64, 128 or 256 rows): the waves share out the rows and all read one key tile, which the whole
 // workgroup brings into LDS, so that a cached byte is dequantised once for all rows.
 //
-// What bounds it (measured, Llama-3-8B layer shape H 32 / KVH 8 / head_dim 128 unless said otherwise): 64 sequences of 4 - 16
-// drafted tokens over 256 - 4 096 keys 119 us = 3.2 TB/s, of it 10 us of partial results in the merge; 16 sequences of 64
-// tokens over 1 k - 8 k keys 116 us = 587 TFLOP/s; 8 sequences of 24 tokens over 32 k - 128 k keys at H 8 / KVH 1 141 us =
-// 531 TFLOP/s, 1.7 TB/s. Per key tile and wave (two row blocks) the vector ALU is busy for about 650 cycles (weights,
-// dequantisation), the matrix pipe for 512, LDS for 160, and the two waves a SIMD holds overlap them only in part: taking
-// out either product, the exponentials, or the staging shortens a launch by about that part's own time.
+// What bounds it (measured, Llama-3-8B layer shape H 32 / KVH 8 / head_dim 128 unless said otherwise; whole calls in turn,
+// without a profiler): 64 sequences of 4 - 16 drafted tokens over 256 - 4 096 keys 119 us = 3.2 TB/s, of it 10 us of partial
+// results in the merge; 16 sequences of 64 tokens over 1 k - 8 k keys 116 - 118 us = 575 - 585 TFLOP/s; 8 sequences of 24
+// tokens over 32 k - 128 k keys at H 8 / KVH 1 141 - 145 us = 515 - 530 TFLOP/s, 1.7 TB/s. By the counters a SIMD's two waves
+// (two row blocks each) keep the vector ALU busy for 1 440 - 1 510 cycles per key tile (weights, dequantisation; 260 are the
+// issue of matrix instructions) and the matrix pipe for 1 020, of the 3 000 - 3 600 that the tile takes, and the CU's LDS for
+// 910: they overlap only in part. Taking out either product, the exponentials, or the staging shortens a launch by about
+// that part's own time.
 #include "cache_tile.h"
 
 namespace pplhip {
@@ -56,9 +58,12 @@ constexpr int64_t kPieceCost = 4; // what starting and finishing a row tile cost
 // 11.2 at 16 and 32; 24 sequences of up to 1 500 keys and 20 heads: 41.4, 41.0, 51.9 us.
 constexpr int64_t kMinRangeTiles = 16;
 // The reference point m of a row's exponents need not be its running maximum: it only moves when a score passes it by
-// more than 2^kSlack, so that most tiles need neither a maximum across lanes nor a rescaling. Weights are held as
-// exp2(x - m + kProbShift), at most 2^15 in fp16 (the operand of the second product); a weight keeps fp16's full
-// precision down to 2^-22 of 2^m. Sums carry the same factor and keep 32 bits.
+// more than 2^kSlack, so that most tiles need neither a maximum across lanes nor a rescaling. Weights are formed as
+// exp2(x - m + kProbShift), at most 2^15, and enter the second product in fp16: the matrix instructions take both operands
+// in one type, and V is fp16. That rounding, half a step of 2^-10, leaves outputs 2.9e-4 from 64 bits (relative norm) where
+// their own rounding to fp16 makes 2.1e-4; the weights in two fp16 parts would take the second product twice. A weight keeps
+// fp16's full precision down to 2^-22 of 2^m. Sums carry the same factor, are of the weights before that rounding, and keep
+// 32 bits.
 constexpr float kProbShift = 8.f;
 constexpr float kSlack = 7.f;
 
@@ -421,8 +426,11 @@ __device__ inline void walk_range(const TreeParams& p, int range, int kvh, F&& p
     }
 }
 
-// Waves per SIMD that the register allocator is to leave room for: what a wave's N row blocks, the tiles on their way and
-// the operands of one product take without spilling.
+// Waves per SIMD that the register allocator is to leave room for, at least: what a wave's N row blocks, the tiles on their
+// way and the operands of one product take. With fewer channels more of them fit (at 32 and 64 channels up to 7 and 4).
+// The bound costs vector registers spilled at 256 channels (40 and 63 with 16 and 32 rows, 31 and 4 with 64 and 128) and a
+// few in <224> with 32 rows (9) and <128> with 64 (2); the four-wave kernels keep 16 and 40 bytes per lane of the tiles on
+// their way in scratch at 32 and 64 channels.
 constexpr int tree_waves_per_simd(int dh, int row_blocks) {
     return row_blocks == 1 ? (dh <= 128 ? 3 : 2) : (dh <= 128 ? 2 : 1);
 }
@@ -798,16 +806,17 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeParams p, con
 
 // The longest sequence's (token, shared head) rows decide the row tile: the smallest that holds them, so that the cache is
 // read and dequantised once; 256 at most, 128 above head_dim 128, where eight waves of two row blocks do not fit a CU's
-// registers. Measured: 64 rows in tiles of 64 / of 32 (tree_keys_kernel) 173 / 217 us on the serving batch above, 256 rows
-// in tiles of 256 / of 128 124 / 147 us, 192 rows 144 / 194 us. Up to 32 rows the other way round: tiles of 64 would leave
-// all waves but one or two without rows, where tree_keys_kernel gives each a quarter of the keys.
+// registers. Measured: up to 64 rows in tiles of 64 / of 32 (tree_keys_kernel) 119 / 158 us on the serving batch above, 256
+// rows in tiles of 256 / of 128 117 / 145 us, 192 rows 144 / 174 us. Up to 32 rows the other way round: tiles of 64 would
+// leave all waves but one or two without rows, where tree_keys_kernel gives each a quarter of the keys.
 int tree_row_tile(const pplhip_tree_attention_args* a) {
     const int64_t rows = a->max_seqlen * (a->num_heads / a->num_kv_heads);
     return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 || a->head_dim > 128 ? 128 : 256;
 }
 
-// As many ranges as workgroups are resident, shared out among the kv heads (twice as many, with eight waves a workgroup:
-// 147 against 126 us on 256 rows, 203 against 171 us on 192 rows over long contexts); never more than ranges of the least
+// As many ranges as workgroups fit a CU at the waves per SIMD asked for above (where more are resident, at 32 and 64
+// channels, those have no range), shared out among the kv heads (twice as many, with eight waves a workgroup, when the
+// kernels took 126 and 171 us: 147 on 256 rows, 203 on 192 rows over long contexts); never more than ranges of the least
 // length in the longest possible axis.
 int64_t tree_num_ranges(const pplhip_tree_attention_args* a, int cu_count) {
     const int64_t rep = a->num_heads / a->num_kv_heads;
