@@ -82,25 +82,6 @@ __device__ inline void wave_lds_order() {
     __builtin_amdgcn_wave_barrier();
 }
 
-// The largest of four values held by lanes l, l ^ 16, l ^ 32, l ^ 48 (every lane gets it), and their sum: the swap
-// instructions hand every lane of a row pair both rows' values without a trip through LDS.
-__device__ inline float max_over_groups(float v) {
-    const uint32_t u = __float_as_uint(v);
-    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    const uint32_t w = __float_as_uint(v);
-    const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
-    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-__device__ inline float sum_over_groups(float v) {
-    const uint32_t u = __float_as_uint(v);
-    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-    const uint32_t w = __float_as_uint(v);
-    const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
-    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
-
 // |int8| <= 128, and 128 * 511 is below fp16's largest: such a group's values are finite
 __device__ inline bool scale_is_small(half_t s) {
     return __builtin_fabsf((float)s) < 511.f;

@@ -120,27 +120,6 @@ typedef const int64_t __attribute__((address_space(4)))* const_tab_t;
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 typedef const __attribute__((address_space(1))) void* gbl_ptr_t;
 
-// Reductions over the four 16-lane rows of the wave (lanes l, l^16, l^32, l^48) in the vector ALU: the swap
-// instructions hand every lane of a row pair both rows' values, where a shuffle would be a round trip through the LDS
-// pipeline. v_permlane16_swap(x, y) exchanges the odd rows of x with the even rows of y; v_permlane32_swap(x, y) the
-// upper half of x with the lower half of y; with x = y = v the two results hold the two partners' values.
-__device__ inline float wave_max_over_quads(float v) {
-    const uint32_t u = __float_as_uint(v);
-    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    const uint32_t w = __float_as_uint(v);
-    const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
-    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-__device__ inline float wave_sum_over_quads(float v) {
-    const uint32_t u = __float_as_uint(v);
-    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-    const uint32_t w = __float_as_uint(v);
-    const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
-    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
-
 // Pins a pointer that is wave-uniform by construction into scalar registers, so that memory instructions take the
 // "scalar base + 32-bit lane offset" addressing form.
 __device__ inline const char* make_uniform(const char* p) {

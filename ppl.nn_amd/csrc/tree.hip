@@ -265,7 +265,7 @@ struct RowState {
     __device__ inline void settle(float scale_log2, const float (&top)[N]) {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const float m_new = fmaxf(m[n], max_over_groups(top[n]));
+            const float m_new = fmaxf(m[n], wave_max_over_quads(top[n]));
             const float ref = m_new == -INFINITY ? 0.f : m_new;
             const float alpha = __builtin_amdgcn_exp2f((m[n] - ref) * scale_log2);
             m[n] = m_new;
@@ -531,7 +531,7 @@ __global__ __launch_bounds__(256, tree_waves_per_simd(DH, NR)) void tree_keys_ke
         const int tid = recomputed(threadIdx.x), r_lane = tid & 15, g = (tid & 63) >> 4;
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
-            const float l = sum_over_groups(st.l[n]);
+            const float l = wave_sum_over_quads(st.l[n]);
             if (g == 0) ml_lds[wave][16 * n + r_lane] = make_float2(st.m[n] * p.scale_log2, l);
         }
         __syncthreads();
@@ -724,7 +724,7 @@ __global__ __launch_bounds__(W * 64, tree_waves_per_simd(DH, NB)) void tree_rows
         const int lane = recomputed(threadIdx.x & 63), g = lane >> 4;
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
-            const float l = sum_over_groups(st.l[n]);
+            const float l = wave_sum_over_quads(st.l[n]);
             const int r = 16 * (wave + W * n) + (lane & 15); // within the tile
             if (t.whole) {
 #pragma unroll
